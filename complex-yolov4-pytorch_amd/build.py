@@ -10,6 +10,10 @@ INCLUDE = os.path.join(HERE, '..', 'include')
 LIB = os.path.join(CSRC, 'libcyolo_hip.so')
 SOURCES = ['conv_igemm.hip', 'conv_pipe.hip', 'conv_direct.hip', 'conv_wgrad.hip', 'elementwise.hip', 'yolo_head.hip', 'riou_nms.hip', 'bev.hip']
 HEADERS = ['common.hpp', 'igemm_common.hpp', 'geometry.hpp', os.path.join(INCLUDE, 'cyolo_hip.h')]
+# Per-image layers (group norm, dropout): kernels nothing times or tunes, so they are not part of the sources the persisted conv choices
+# are stamped with (tune.py: csrc/*.h*) -- an edit here leaves that table valid.
+LAYER_SOURCES = ['layers/group_norm.hip', 'layers/dropout.hip']
+LAYER_HEADERS = ['layers/layer_common.hpp']
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + INCLUDE, '-I' + CSRC, '-Wno-unused-value']
 # Per-file flags.  yolo_head.hip / riou_nms.hip: the per-target / per-pair kernels index small polygon arrays dynamically; with the
 # default promote-alloca budget they lived in scratch memory (368 / 880 bytes per lane) and assign / pairs were the only kernels of
@@ -31,12 +35,14 @@ _NO_SLP = ['-fno-slp-vectorize']
 _NO_SLP_FILES = ('yolo_head.hip', 'riou_nms.hip', 'bev.hip')
 EXTRA_FLAGS = {src: _REMARKS + (_ALLOCA if src in ('yolo_head.hip', 'riou_nms.hip') else []) +
                (_NO_SLP if (src in _NO_SLP_FILES or os.environ.get('CY_BUILD_NO_SLP') == '1') else []) for src in SOURCES}
+# Packed float32 instructions are switched off in the layer kernels altogether: they run beside the weight-gradient stream's MFMA waves.
+LAYER_FLAGS = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops'] + _REMARKS
 # NO kernel of the library may come out of the compiler with a private segment (scratch): checked on every compile of every
 # file (check_scratch).  Round 2 found the head kernels' results to depend on what ran beside them while they spilled; round 3
 # found two conv instantiations that had quietly acquired spills (a 384 x 128 direct-store epilogue, 196 bytes per lane) while
 # hunting a 1-in-10^4 gradient difference of the deterministic mode.  A different hipcc or a small edit can bring a spill
 # back silently -- with this check it fails the build instead.  '*' = every kernel of the file.
-NO_SCRATCH = {src: ('*',) for src in SOURCES}
+NO_SCRATCH = {src: ('*',) for src in SOURCES + LAYER_SOURCES}
 RESOURCES = os.path.join(CSRC, 'kernel_resources.json')
 
 
@@ -138,12 +144,14 @@ def build(force=False, verbose=False):
                                '-I' + os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(hipcc))), 'include'),
                                '-D__HIP_PLATFORM_AMD__', '-x', 'c++',
                                '-c', PLAN_SRC, '-o', plan_o])
-    for src in SOURCES:
+    layer_time = max([hdr_time] + [_mtime(os.path.join(CSRC, h)) for h in LAYER_HEADERS])
+    for src in SOURCES + LAYER_SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(CSRC, src.replace('.hip', '.o'))
         objs.append(o)
-        if force or _mtime(o) < max(_mtime(s), hdr_time, _mtime(os.path.abspath(__file__))):      # (this file holds the per-file flags)
-            cmd = [hipcc] + FLAGS + EXTRA_FLAGS.get(src, []) + ['-c', s, '-o', o]
+        newest = layer_time if src in LAYER_SOURCES else hdr_time
+        if force or _mtime(o) < max(_mtime(s), newest, _mtime(os.path.abspath(__file__))):      # (this file holds the per-file flags)
+            cmd = [hipcc] + FLAGS + (LAYER_FLAGS if src in LAYER_SOURCES else EXTRA_FLAGS.get(src, [])) + ['-c', s, '-o', o]
             if verbose:
                 print(' '.join(cmd))
             procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))

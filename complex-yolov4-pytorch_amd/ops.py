@@ -556,6 +556,119 @@ def bn_act_bwd_apply(x, dy, dx, res_grad, res_accum, mean, invstd, scale, shift,
                _p(shift), _p(dgs), _p(dbs), act, x.dt, _stream())
 
 
+# ---- per-image layers: group norm + activation, dropout ---------------------------------------------
+
+def _check_layer(who, first, views=(), floats=(), rng=None):
+    """Arguments of the per-image layers: views of one shape, type and device, float32 vectors of given sizes on that device, and
+    that device the current one (the launch goes to its current stream)."""
+    _require_gpu()
+    dev = first.buf.device
+    check_device_tensor(first.buf, who)
+    if dev.index != torch.cuda.current_device():
+        raise CyoloError('%s: the tensors are on %s, the current device is cuda:%d' % (who, dev, torch.cuda.current_device()))
+    dt = _TORCH_DT.get(first.dt)
+    for v in (first,) + tuple(views):
+        if v is None:
+            continue
+        if (v.N, v.H, v.W, v.C, v.dt) != (first.N, first.H, first.W, first.C, first.dt) or v.buf.dtype != dt or v.buf.device != dev:
+            raise CyoloError('%s: views differ in shape, type or device: %s and %s' % (who, _view_str(first), _view_str(v)))
+        if v.ld < v.C or v.off < 0 or (v.M and v.off + (v.M - 1) * v.ld + v.C > v.buf.numel()) or not v.buf.is_contiguous():
+            raise CyoloError('%s: %s reaches beyond its buffer of %d elements' % (who, _view_str(v), v.buf.numel()))
+    for name, t, n in floats:
+        if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.device != dev or not t.is_contiguous()):
+            raise CyoloError('%s: %s must be %d contiguous float32 values on %s' % (who, name, n, dev))
+    if rng is not None and (rng.dtype != torch.int64 or rng.numel() != 2 or rng.device != dev or not rng.is_contiguous()):
+        raise CyoloError('%s: the generator state is a contiguous int64 tensor (seed, step) on %s (ops.dropout_state)' % (who, dev))
+
+
+def _view_str(v):
+    return '[%d, %d, %d, %d] (row stride %d, %s on %s)' % (v.N, v.H, v.W, v.C, v.ld, v.buf.dtype, v.buf.device)
+
+
+def dropout_q(p):
+    """Drop probability -> 65536ths, the resolution of the generator's half-words (cy_dropout)."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise CyoloError('a drop probability lies between 0 and 1, got %r' % p)
+    return int(p * 65536.0 + 0.5)
+
+
+def dropout_state(seed, device='cuda', step=0):
+    """The generator's device state (seed, step).  A training loop adds one to ``state[1]`` before every forward pass."""
+    seed = int(seed) & 0xFFFFFFFFFFFFFFFF
+    return torch.tensor([seed - (1 << 64) if seed >> 63 else seed, int(step)], dtype=torch.int64, device=device)
+
+
+def _drop_args(who, p, rng):
+    q = dropout_q(p)
+    if q and rng is None:
+        raise CyoloError('%s: dropout needs the generator state (ops.dropout_state)' % who)
+    return q
+
+
+def gn_workspace(N, H, W, C, groups, dt, device='cuda'):
+    """Scratch of gn_act_fwd / gn_act_bwd for one shape (contents arbitrary; one per stream that may run them at the same time)."""
+    n = int(lib().raw('cy_gn_workspace')(N, H * W, C, groups, dt))
+    if n < 0:
+        raise CyoloError('cy_gn_workspace: %d channels in %d groups (N %d, %d x %d, type %r)' % (C, groups, N, H, W, dt))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _check_gn(who, x, views, gamma, beta, stats, groups, act, ws, more=(), rng=None):
+    if groups < 1 or x.C % groups:
+        raise CyoloError('%s: %d channels do not divide into %d groups' % (who, x.C, groups))
+    if act not in (0, 1, 2):
+        raise CyoloError('%s: unsupported activation %r' % (who, act))
+    if gamma is None or beta is None:
+        raise CyoloError('%s: scale and shift are needed' % who)
+    _check_layer(who, x, views, (('gamma', gamma, x.C), ('beta', beta, x.C), ('stats', stats, 2 * x.N * groups)) + more, rng)
+    if ws is None or ws.device != x.buf.device or not ws.is_contiguous():
+        raise CyoloError('%s: the workspace is a contiguous tensor on %s (ops.gn_workspace)' % (who, x.buf.device))
+
+
+def gn_act_fwd(x, y, res, gamma, beta, groups, eps, act, stats, ws, drop=0.0, rng=None, drop_id=0):
+    """y = res + dropout(act(group norm of x)); stats: float32 [N, groups, 2] (mean, 1 / deviation) for gn_act_bwd, or None."""
+    _check_gn('gn_act_fwd', x, (y, res), gamma, beta, stats, groups, act, ws, rng=rng)
+    if not eps >= 0.0:
+        raise CyoloError('gn_act_fwd: eps %r' % eps)
+    q = _drop_args('gn_act_fwd', drop, rng)
+    lib().call('cy_gn_act_fwd', _p(x), x.ld, _p(y), y.ld, _p(res), res.ld if res is not None else 0, x.N, x.H * x.W, x.C, groups, _p(gamma),
+               _p(beta), float(eps), act, x.dt, _p(stats), q, _p(rng), int(drop_id), _p(ws), ws.numel() * ws.element_size(),
+               _stream())
+
+
+def gn_act_bwd(x, dy, dx, res_grad, res_accum, gamma, beta, stats, groups, act, ggamma, gbeta, gscale, accumulate, ws, drop=0.0, rng=None,
+               drop_id=0):
+    """dx (may be dy), ggamma / gbeta (+)= gscale * sums (None: not wanted); res_grad (+)= dy, the shortcut branch's gradient."""
+    if stats is None:
+        raise CyoloError('gn_act_bwd: the statistics of the forward pass are needed')
+    _check_gn('gn_act_bwd', x, (dy, dx, res_grad), gamma, beta, stats, groups, act, ws,
+              (('ggamma', ggamma, x.C), ('gbeta', gbeta, x.C)), rng)
+    q = _drop_args('gn_act_bwd', drop, rng)
+    lib().call('cy_gn_act_bwd', _p(x), x.ld, _p(dy), dy.ld, _p(dx), dx.ld, _p(res_grad), res_grad.ld if res_grad is not None else 0,
+               int(bool(res_accum)), x.N, x.H * x.W, x.C, groups, _p(gamma), _p(beta), _p(stats), act, x.dt, _p(ggamma), _p(gbeta),
+               float(gscale), int(bool(accumulate)), q, _p(rng), int(drop_id), _p(ws), ws.numel() * ws.element_size(), _stream())
+
+
+def dropout_fwd(x, y, p, rng, drop_id=0):
+    """y = kept ? x / (1 - p) : 0 (y may be x); the mask is a function of (rng, drop_id, element index) and is never stored."""
+    _check_layer('dropout_fwd', x, (y,), rng=rng)
+    _dropout('dropout_fwd', x, y, p, rng, drop_id, False)
+
+
+def dropout_bwd(dy, dx, accumulate, p, rng, drop_id=0):
+    """dx (+)= the same map of dy."""
+    _check_layer('dropout_bwd', dy, (dx,), rng=rng)
+    _dropout('dropout_bwd', dy, dx, p, rng, drop_id, accumulate)
+
+
+def _dropout(who, x, y, p, rng, drop_id, accumulate):
+    if rng is None:
+        raise CyoloError('%s: dropout needs the generator state (ops.dropout_state)' % who)
+    q = dropout_q(p)
+    lib().call('cy_dropout', _p(x), x.ld, _p(y), y.ld, x.M, x.C, q, _p(rng), int(drop_id), int(bool(accumulate)), x.dt, _stream())
+
+
 def maxpool_argmax_bytes(N, H, OH, OW, C):
     return int(lib().raw('cy_maxpool_argmax_bytes')(N, H, OH, OW, C))
 

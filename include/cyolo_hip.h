@@ -311,6 +311,45 @@ int cy_bn_act_bwd_apply(const void* x, int ldx, const void* dy, int lddy, void* 
                         const float* scale, const float* shift, const float* dgamma_sum, const float* dbeta_sum,
                         int act, int dtype, cy_stream_t s);
 
+/* ------------------------------------------------------------------------------------------------
+ * Per-image layers (no counterpart in the reference's cfgs: Darknet's [dropout] block and group normalisation as a
+ * replacement of the batch's statistics where a GPU holds one or two images)
+ * ---------------------------------------------------------------------------------------------- */
+
+/* Group normalisation + activation (+ dropout) (+ shortcut) over a view of N images x HW pixels x C channels, G = groups sets
+ * of C / G consecutive channels:
+ *   mean, var of one image's pixels and one group's channels (biased),  r = 1 / sqrt(var + eps)
+ *   y = res + drop(act(gamma[c] * (x - mean) * r + beta[c]))
+ * The same function in training and in eval mode; stats (may be NULL: eval) receives (mean, r) as float [N][groups][2], 8-byte
+ * aligned, for the backward pass.  res may be NULL.  Any C divisible by groups, any row strides >= C, any element-aligned pointer
+ * (rows that all start on 16 bytes take the fast kernels).  y may be x (every element is read before it is written by the same
+ * thread); no other overlap.  N = 0 or HW = 0: nothing to do.
+ * Dropout (see cy_dropout): q > 0 drops with probability q / 65536, rng / id as there; element index = ((n * HW + pixel) * C + c).
+ * ws: cy_gn_workspace() bytes, 8-byte aligned, contents arbitrary; used by the call from its first to its last launch (calls on
+ * different streams, captured graphs that may run at the same time among them, need one each).
+ * No atomics: results are bit-identical from run to run. */
+int cy_gn_act_fwd(const void* x, int ldx, void* y, int ldy, const void* res, int ldres, int N, int64_t HW, int C, int groups,
+                  const float* gamma, const float* beta, float eps, int act, int dtype, float* stats, int q, const int64_t* rng,
+                  int id, void* ws, int64_t ws_bytes, cy_stream_t s);
+/* Backward of the above: dx from x, dy and the forward pass's stats (same gamma, beta, act, q, rng contents, id); dx may be dy.
+ * When res_grad is non-NULL the shortcut branch's gradient, dy itself, is added into it (res_accum) or stored.
+ * ggamma / gbeta (either may be NULL): gscale * sum, added (accumulate) or stored. */
+int cy_gn_act_bwd(const void* x, int ldx, const void* dy, int lddy, void* dx, int lddx, void* res_grad, int ldrg, int res_accum,
+                  int N, int64_t HW, int C, int groups, const float* gamma, const float* beta, const float* stats, int act,
+                  int dtype, float* ggamma, float* gbeta, float gscale, int accumulate, int q, const int64_t* rng, int id,
+                  void* ws, int64_t ws_bytes, cy_stream_t s);
+/* Bytes of ws for either call. */
+int64_t cy_gn_workspace(int N, int64_t HW, int C, int groups, int dtype);
+
+/* Dropout over a view of M pixels x C channels, the mask never stored:
+ *   y = keep[e] ? x * 65536 / (65536 - q) : 0     (accumulate: added to what y holds)
+ * e = pixel * C + c; keep[e] = half-word e % 8 (low half of word 0 first) of the Philox-4x32-10 block e / 8 is >= q, with
+ *   key = (low, high word of rng[0]), counter = (low, high word of e / 8, low word of rng[1], id)
+ * -- rng: device int64 [2] = (seed, step); id tells the layers of a network apart.  0 <= q <= 65536 (65536: everything is dropped;
+ * a dropped NaN is 0).  The backward pass is the same call on dy.  Any strides >= C and element-aligned pointers; y may be x. */
+int cy_dropout(const void* x, int ldx, void* y, int ldy, int64_t M, int C, int q, const int64_t* rng, int id, int accumulate,
+               int dtype, cy_stream_t s);
+
 /* Data-movement blocks of Darknet.forward (darknet2pytorch.py:180-219, :64-79, :285). */
 /* Max pooling (SPP 5/9/13 stride 1, tiny's 2x2 stride 2) as a row pass and a column pass (k + k loads per output, torch's
  * value and tie rule).  `scratch`: >= N*H*OW*C elements of the tensor dtype (forward) / floats (backward).  `argmax`
