@@ -1,0 +1,110 @@
+// Arithmetic that every group norm kernel shares.
+//
+// These kernels stand or fall with the number of vector instructions per element: a wave's instruction takes four cycles, so 256
+// compute units do 39e12 of them a second, and at 16-bit storage memory asks for an element every 0.7 ps forward (4 bytes) and 1.1 ps
+// backward (6 bytes): 27 and 43 instructions.
+#pragma once
+#include "layer_common.hpp"
+
+// The value as it stands: keeps the conversion to 16 bits that follows from being merged into the multiply-add before it (one rounding
+// instead of two, where the compiler finds it: two kernels' stored values would differ in their last bit).
+__device__ __forceinline__ float rounded(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
+// ---- normalisation -----------------------------------------------------------------------------------------------------------
+// Per channel, from the group's (mean, r) and (gamma, beta): z(x) and the deviation from the mean.
+//
+// LEAKY: d = x - mean, xh = d r, z = gamma xh + beta, every operation rounded (no contraction): which side of the kink a value falls on
+// is then a function of the inputs and the statistics alone, the same in the forward and the backward pass and in every kernel.
+// Smooth activations: z = x (gamma r) + (beta - mean gamma r), one multiply-add (for f16 straight from the stored half).  With 16-bit
+// storage the rounding of the shift, |mean| 2^-24, is at most 2^-13 of the step in which x itself is stored beside that mean; in 32
+// bits the deviation is formed first.
+template <typename T, int ACT>
+struct Norm {
+    static constexpr bool DIRECT = sizeof(T) == 2 && ACT != CY_ACT_LEAKY;
+    float mean, r, ga, be;      // DIRECT: ga = gamma r, be = beta - mean gamma r
+    __device__ __forceinline__ void set(float2 stat, float gamma, float beta) {
+#pragma clang fp contract(off)
+        mean = stat.x;
+        r = stat.y;
+        ga = DIRECT ? gamma * stat.y : gamma;
+        be = DIRECT ? fmaf(-stat.x, ga, beta) : beta;
+    }
+    __device__ __forceinline__ float z(float x) const {
+#pragma clang fp contract(off)
+        if constexpr (DIRECT) return ACT == CY_ACT_LINEAR ? rounded(fmaf(x, ga, be)) : fmaf(x, ga, be);
+        const float d = x - mean;
+        const float xh = d * r;
+        const float g = xh * ga;
+        return g + be;
+    }
+};
+
+// dx = r (gamma dz - S1 - xh S2) = dz (gamma r) + (x - mean) k1 + k0, with (k0, k1) = (-r S1, -r^2 S2) of the group
+__device__ __forceinline__ float2 gn_k01(float r, double s1, double s2) {
+#pragma clang fp contract(off)
+    return make_float2(-r * (float)s1, -r * (r * (float)s2));
+}
+template <typename T, int ACT>
+__device__ __forceinline__ float gn_dx(const Norm<T, ACT>& nm, float2 k, float x, float dz) {
+#pragma clang fp contract(off)
+    const float k2 = Norm<T, ACT>::DIRECT ? nm.ga : nm.ga * nm.r;
+    return rounded(fmaf(dz, k2, fmaf(x - nm.mean, k.y, k.x)));
+}
+
+// ---- activations -------------------------------------------------------------------------------------------------------------
+// mish(z) = z tanh(log(1 + e^z)).  With n = e^z, w = n (n + 2): tanh = w / (w + 2).  FAST (16-bit storage): hardware exponential and
+// reciprocal, 1 - 2 e each; the exponent is clamped where w / (w + 2) is 1 in 32 bits and w still finite, so no value needs a branch.
+// Derivative: with q = 2 / (w + 2) = 1 - tanh it is (1 - q) + z q^2 (w - n): one exponential, one reciprocal.
+// (No contraction is left to the compiler anywhere in this file: a value comes out the same wherever it is computed, by the block that
+// holds it or by the one that finishes for it.)
+constexpr float LOG2E = 1.44269504088896341f;
+template <bool FAST>
+__device__ __forceinline__ float gn_exp(float z) {      // e^z, at most 2^30
+    return FAST ? __builtin_amdgcn_exp2f(fminf(z * LOG2E, 30.f)) : expf(fminf(z, 20.f));
+}
+template <int ACT, bool FAST>
+__device__ __forceinline__ float gn_act(float z) {
+#pragma clang fp contract(off)
+    if constexpr (ACT == CY_ACT_MISH) {
+        const float n = gn_exp<FAST>(z);
+        const float w = n * (n + 2.f);
+        return z * (FAST ? w * __builtin_amdgcn_rcpf(w + 2.f) : w / (w + 2.f));
+    }
+    return ACT == CY_ACT_LEAKY && !(z > 0.f) ? 0.1f * z : z;
+}
+template <int ACT, bool FAST>
+__device__ __forceinline__ float gn_act_grad(float z) {
+#pragma clang fp contract(off)
+    if constexpr (ACT == CY_ACT_MISH) {
+        const float n = gn_exp<FAST>(z);
+        const float w = n * (n + 2.f);
+        if constexpr (FAST) {
+            const float q = __builtin_amdgcn_rcpf(fmaf(w, 0.5f, 1.f));
+            return fmaf(z * (w - n), q * q, 1.f - q);
+        }
+        const float t = w / (w + 2.f), q = 2.f / (w + 2.f);
+        return fmaf(z * (w - n), q * q, t);      // (32 bits: tanh by itself, 1 - q cancels for large negative z)
+    }
+    return ACT == CY_ACT_LEAKY && !(z > 0.f) ? 0.1f : 1.f;
+}
+
+__device__ __forceinline__ float gn_rstd(double var, float eps) {
+    if (var < 0.0) var = 0.0;
+    return (float)(1.0 / sqrt(var + (double)eps));
+}
+
+// ---- statistics --------------------------------------------------------------------------------------------------------------
+// How many sums a thread keeps for the V channels of a chunk: 1 -- they lie in one group (Cg % V == 0); V / Cg -- one for each of the whole
+// groups in the chunk; V -- one per channel.
+template <int V>
+static inline int gn_sums(int Cg) {
+    return Cg % V == 0 ? 1 : V % Cg == 0 ? V / Cg : V;
+}
+// columns (thread sums side by side) of a group
+template <int V>
+__device__ __host__ static inline int gn_cols(int Cg) {
+    return Cg % V == 0 ? Cg / V : V % Cg == 0 ? 1 : Cg;
+}

@@ -5,11 +5,13 @@
 //   dz = drop(dy) act'(z),  xh = (x - mean) r,   dbeta = sum dz,  dgamma = sum dz xh
 //   dx = r (gamma dz - S1 - xh S2),   S1, S2 = group means of gamma dz and gamma dz xh
 //
-// Three launches per direction: partial sums per (image, pixel range, column), a fold, the element pass.  No atomics: a call's
-// results do not depend on scheduling.
+// This file: the choice of kernels, the C entry points, and the general kernels -- three launches per direction: partial sums per
+// (image, pixel range, column), a fold, the element pass -- for any row stride, alignment and channel count.  The one-launch kernels
+// are in gn_resident_*.  No floating-point atomics anywhere: a call's results do not depend on scheduling.
 //
 // A block works on one image n, one span of chunk columns and one range of pixels; thread = (row = t / width, chunk = t % width).
-#include "layer_common.hpp"
+#include "gn_math.hpp"
+#include "gn_resident.hpp"
 
 namespace {
 
@@ -44,8 +46,12 @@ __device__ __forceinline__ Where where(const Shape& sh) {
     return w;
 }
 
-// smallest power of two >= n
-__device__ __forceinline__ int pow2_up(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
+// A thread requests U pixels before it looks at the first.  Pixels behind the block's range are read as its last one and left out
+// afterwards: no branch between the loads.
+__device__ __forceinline__ long pixel(long p, int u, const Where& w) {
+    const long q = p + (long)u * w.rows;
+    return q < w.p1 ? q : w.p1 - 1;
+}
 
 // Statistics of a column: NACC = 1 -- a chunk lies in one group, one (mean, sum of squares) per thread; NACC = V -- one per channel.
 // Every thread sums deviations from the FIRST value it reads: that value is one of the column's own, so the square of its distance
@@ -53,6 +59,7 @@ __device__ __forceinline__ int pow2_up(int n) { return n <= 1 ? 1 : 1 << (32 - _
 // of values a thread holds -- whatever the mean of the data.  Threads are merged by mean and centred sum of squares.
 template <typename T, int V, int NACC>
 __global__ void __launch_bounds__(256) gn_stats_kernel(const T* x, int ldx, Shape sh, float* part) {
+    constexpr int U = 8;
     __shared__ float s_m[256 * NACC], s_q[256 * NACC], s_n[256];
     const Where w = where(sh);
     float K[NACC], s[NACC], q[NACC];
@@ -61,20 +68,29 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const T* x, int ldx, Shap
     int cnt = 0;
     if (w.on) {
         const T* src = x + (long)w.n * sh.HW * ldx + w.chunk * V;
-        for (long p = w.p0 + w.row; p < w.p1; p += w.rows) {
-            float f[V];
-            load_v<T, V>(src + p * ldx, f);
+        for (long p = w.p0 + w.row; p < w.p1; p += (long)U * w.rows) {
+            Raw<T, V> in[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) in[u].load(src + pixel(p, u, w) * ldx);
             if (cnt == 0) {
+                float f[V];
+                in[0].get(f);
 #pragma unroll
                 for (int a = 0; a < NACC; ++a) K[a] = f[a];
             }
-            ++cnt;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int a = NACC == 1 ? 0 : i;
-                const float d = f[i] - K[a];
-                s[a] += d;
-                q[a] += d * d;
+            for (int u = 0; u < U; ++u) {
+                if (p + (long)u * w.rows >= w.p1) break;
+                float f[V];
+                in[u].get(f);
+                ++cnt;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const int a = NACC == 1 ? 0 : i;
+                    const float d = f[i] - K[a];
+                    s[a] += d;
+                    q[a] += d * d;
+                }
             }
         }
     }
@@ -146,81 +162,62 @@ __global__ void __launch_bounds__(256) gn_fold_kernel(const float* part, Shape s
     }
     m2 = wave_sum_d(m2);
     if (lane == 0) {
-        double var = m2 / (total * per_col);
-        if (var < 0.0) var = 0.0;
         stats[2 * job] = (float)mean;
-        stats[2 * job + 1] = (float)(1.0 / sqrt(var + (double)eps));
+        stats[2 * job + 1] = gn_rstd(m2 / (total * per_col), eps);
     }
-}
-
-// act < 0: chosen at run time (the one-element kernels)
-template <int ACT, bool FAST>
-__device__ __forceinline__ float act_any(float z, int act) {
-    if constexpr (ACT >= 0) return act_f<ACT, FAST>(z);
-    else return act == CY_ACT_MISH ? act_f<CY_ACT_MISH, FAST>(z) : act == CY_ACT_LEAKY ? act_f<CY_ACT_LEAKY, FAST>(z) : z;
-}
-template <int ACT, bool FAST>
-__device__ __forceinline__ float act_grad_any(float z, int act) {
-    if constexpr (ACT >= 0) return act_grad<ACT, FAST>(z);
-    else return act == CY_ACT_MISH ? act_grad<CY_ACT_MISH, FAST>(z) : act == CY_ACT_LEAKY ? act_grad<CY_ACT_LEAKY, FAST>(z) : 1.f;
-}
-
-// xh = (x - mean) r and z = gamma xh + beta with every operation rounded (no contraction), in both directions: which side of the leaky
-// activation's kink a value falls on is then a function of the inputs and the statistics alone, the same in the forward and the
-// backward pass.  (The mean is subtracted first: folding it into the shift loses |mean| / deviation in accuracy.)
-__device__ __forceinline__ float norm_xh(float x, float mean, float r) {
-#pragma clang fp contract(off)
-    const float d = x - mean;
-    return d * r;
-}
-__device__ __forceinline__ float norm_z(float xh, float gamma, float beta) {
-#pragma clang fp contract(off)
-    const float g = xh * gamma;
-    return g + beta;
 }
 
 template <typename T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) gn_apply_kernel(const T* x, int ldx, T* y, int ldy, const T* res, int ldres, Shape sh,
-                                                      const float* stats, const float* gamma, const float* beta, int act,
+                                                      const float* stats, const float* gamma, const float* beta,
                                                       DropRng rng) {
     constexpr bool FAST = sizeof(T) == 2;
+    constexpr int U = 4;
     const Where w = where(sh);
     if (!w.on) return;
     DropKey key;
     if constexpr (DROP) key = drop_key(rng);
-    float mu[V], rs[V], ga[V], be[V];
+    Norm<T, ACT> nm[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = w.chunk * V + i;
-        const float* st = stats + 2 * ((long)w.n * sh.G + c / sh.Cg);
-        mu[i] = st[0];
-        rs[i] = st[1];
-        ga[i] = gamma[c];
-        be[i] = beta[c];
+        nm[i].set(*reinterpret_cast<const float2*>(stats + 2 * ((long)w.n * sh.G + c / sh.Cg)), gamma[c], beta[c]);
     }
-    for (long p = w.p0 + w.row; p < w.p1; p += w.rows) {
-        const long px = (long)w.n * sh.HW + p;
-        float f[V];
-        load_v<T, V>(x + px * ldx + w.chunk * V, f);
+    const long img = (long)w.n * sh.HW;
+    for (long p = w.p0 + w.row; p < w.p1; p += (long)U * w.rows) {
+        Raw<T, V> in[U], rin[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = act_any<ACT, FAST>(norm_z(norm_xh(f[i], mu[i], rs[i]), ga[i], be[i]), act);
-        if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, f);
+        for (int u = 0; u < U; ++u) in[u].load(x + (img + pixel(p, u, w)) * ldx + w.chunk * V);
         if (res) {
-            float r[V];
-            load_v<T, V>(res + px * ldres + w.chunk * V, r);
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] += r[i];
+            for (int u = 0; u < U; ++u) rin[u].load(res + (img + pixel(p, u, w)) * ldres + w.chunk * V);
         }
-        store_v<T, V>(y + px * ldy + w.chunk * V, f);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (p + (long)u * w.rows >= w.p1) break;
+            const long px = img + p + (long)u * w.rows;
+            float f[V];
+            in[u].get(f);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = gn_act<ACT, FAST>(nm[i].z(f[i]));
+            if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, f);
+            if (res) {
+                float r[V];
+                rin[u].get(r);
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] += r[i];
+            }
+            store_v<T, V>(y + px * ldy + w.chunk * V, f);
+        }
     }
 }
 
 // Partial sums of dz and dz * xh per (image, pixel range, channel)
 template <typename T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const T* x, int ldx, const T* dy, int lddy, Shape sh, const float* stats,
-                                                         const float* gamma, const float* beta, int act, DropRng rng,
-                                                         float* part) {
+                                                         const float* gamma, const float* beta, DropRng rng, float* part) {
     constexpr bool FAST = sizeof(T) == 2;
+    constexpr int U = 4;
     __shared__ float red[256 * V * 2];
     const Where w = where(sh);
     float a[V], b[V];
@@ -229,27 +226,38 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const T* x, int ldx, c
     if (w.on) {
         DropKey key;
         if constexpr (DROP) key = drop_key(rng);
-        float mu[V], rs[V], ga[V], be[V];
+        Norm<T, ACT> nm[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = w.chunk * V + i;
-            const float* st = stats + 2 * ((long)w.n * sh.G + c / sh.Cg);
-            mu[i] = st[0]; rs[i] = st[1]; ga[i] = gamma[c]; be[i] = beta[c];
+            nm[i].set(*reinterpret_cast<const float2*>(stats + 2 * ((long)w.n * sh.G + c / sh.Cg)), gamma[c], beta[c]);
         }
-        for (long p = w.p0 + w.row; p < w.p1; p += w.rows) {
-            const long px = (long)w.n * sh.HW + p;
-            float f[V], g[V];
-            load_v<T, V>(x + px * ldx + w.chunk * V, f);
-            load_v<T, V>(dy + px * lddy + w.chunk * V, g);
-            if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, g);
+        const long img = (long)w.n * sh.HW;
+        for (long p = w.p0 + w.row; p < w.p1; p += (long)U * w.rows) {
+            Raw<T, V> in[U], gin[U];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float xh = norm_xh(f[i], mu[i], rs[i]);
-                const float dz = g[i] * act_grad_any<ACT, FAST>(norm_z(xh, ga[i], be[i]), act);
-                a[i] += dz;
-                b[i] += dz * xh;
+            for (int u = 0; u < U; ++u) {
+                in[u].load(x + (img + pixel(p, u, w)) * ldx + w.chunk * V);
+                gin[u].load(dy + (img + pixel(p, u, w)) * lddy + w.chunk * V);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (p + (long)u * w.rows >= w.p1) break;
+                const long px = img + p + (long)u * w.rows;
+                float f[V], g[V];
+                in[u].get(f);
+                gin[u].get(g);
+                if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, g);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float dz = g[i] * gn_act_grad<ACT, FAST>(nm[i].z(f[i]));
+                    a[i] += dz;
+                    b[i] += dz * (f[i] - nm[i].mean);
+                }
             }
         }
+#pragma unroll
+        for (int i = 0; i < V; ++i) b[i] *= nm[i].r;
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -316,8 +324,9 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const T* x, int ldx, 
                                                           int ldrg, int res_accum, Shape sh, const float* stats,
                                                           const float* gamma, const float* beta, const float* chan,
                                                           const float* s12, float* ggamma, float* gbeta, float gscale,
-                                                          int accumulate, int act, DropRng rng) {
+                                                          int accumulate, DropRng rng) {
     constexpr bool FAST = sizeof(T) == 2;
+    constexpr int U = 4;
     const Where w = where(sh);
     if (!w.on) return;
     if (w.n == 0 && w.blk == 0 && w.row == 0) {      // parameter gradients of this span: image order, double
@@ -335,36 +344,47 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const T* x, int ldx, 
     }
     DropKey key;
     if constexpr (DROP) key = drop_key(rng);
-    float mu[V], rs[V], ga[V], be[V], m1[V], m2[V];
+    Norm<T, ACT> nm[V];
+    float2 k[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = w.chunk * V + i;
         const long j = 2 * ((long)w.n * sh.G + c / sh.Cg);
-        mu[i] = stats[j]; rs[i] = stats[j + 1]; ga[i] = gamma[c]; be[i] = beta[c];
-        m1[i] = s12[j]; m2[i] = s12[j + 1];
+        nm[i].set(*reinterpret_cast<const float2*>(stats + j), gamma[c], beta[c]);
+        k[i] = gn_k01(nm[i].r, s12[j], s12[j + 1]);
     }
-    for (long p = w.p0 + w.row; p < w.p1; p += w.rows) {
-        const long px = (long)w.n * sh.HW + p;
-        float f[V], g[V];
-        load_v<T, V>(x + px * ldx + w.chunk * V, f);
-        load_v<T, V>(dy + px * lddy + w.chunk * V, g);
-        if (resg) {      // the shortcut branch's gradient is dy itself
-            float o[V];
+    const long img = (long)w.n * sh.HW;
+    for (long p = w.p0 + w.row; p < w.p1; p += (long)U * w.rows) {
+        Raw<T, V> in[U], gin[U];
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = 0.f;
-            if (res_accum) load_v<T, V>(resg + px * ldrg + w.chunk * V, o);
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[i] += g[i];
-            store_v<T, V>(resg + px * ldrg + w.chunk * V, o);
+        for (int u = 0; u < U; ++u) {
+            in[u].load(x + (img + pixel(p, u, w)) * ldx + w.chunk * V);
+            gin[u].load(dy + (img + pixel(p, u, w)) * lddy + w.chunk * V);
         }
-        if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, g);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float xh = norm_xh(f[i], mu[i], rs[i]);
-            const float dz = g[i] * act_grad_any<ACT, FAST>(norm_z(xh, ga[i], be[i]), act);
-            f[i] = rs[i] * (ga[i] * dz - m1[i] - xh * m2[i]);
+        for (int u = 0; u < U; ++u) {
+            if (p + (long)u * w.rows >= w.p1) break;
+            const long px = img + p + (long)u * w.rows;
+            float f[V], g[V];
+            in[u].get(f);
+            gin[u].get(g);
+            if (resg) {      // the shortcut branch's gradient is dy itself
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = 0.f;
+                if (res_accum) load_v<T, V>(resg + px * ldrg + w.chunk * V, o);
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] += g[i];
+                store_v<T, V>(resg + px * ldrg + w.chunk * V, o);
+            }
+            if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, g);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float dz = g[i] * gn_act_grad<ACT, FAST>(nm[i].z(f[i]));
+                f[i] = gn_dx(nm[i], k[i], f[i], dz);
+            }
+            store_v<T, V>(dx + px * lddx + w.chunk * V, f);
         }
-        store_v<T, V>(dx + px * lddx + w.chunk * V, f);
     }
 }
 
@@ -406,7 +426,8 @@ int64_t need_floats(const Shape& sh) {
     return 2 * ((int64_t)sh.N * sh.nblk * sh.C + (int64_t)sh.N * sh.G + (int64_t)sh.N * sh.C);
 }
 
-bool grid_ok(const Shape& sh) { return (int64_t)sh.N * sh.nspan * sh.nblk < (1ll << 31) && ((int64_t)sh.N * sh.G + 3) / 4 < (1ll << 31); }
+constexpr int64_t MAX_BLOCKS = 1 << 24;      // a launch has fewer than 2^32 threads
+bool grid_ok(const Shape& sh) { return (int64_t)sh.N * sh.nspan * sh.nblk < MAX_BLOCKS && ((int64_t)sh.N * sh.G + 3) / 4 < MAX_BLOCKS; }
 
 template <typename T, int V>
 int forward(const T* x, int ldx, T* y, int ldy, const T* res, int ldres, const Shape& sh, const float* gamma, const float* beta,
@@ -422,14 +443,13 @@ int forward(const T* x, int ldx, T* y, int ldy, const T* res, int ldres, const S
     hipLaunchKernelGGL(gn_fold_kernel, fgrid, dim3(256), 0, s, part, sh, one ? sh.Cg / V : sh.Cg, one ? V : 1, eps, stats);
     CY_LAUNCH_CHECK();
 #define CY_GNA(A_, D_)                                                                                                         \
-    hipLaunchKernelGGL((gn_apply_kernel<T, V, A_, D_>), grid, dim3(256), 0, s, x, ldx, y, ldy, res, ldres, sh, stats, gamma, beta, act, rng)
+    hipLaunchKernelGGL((gn_apply_kernel<T, V, A_, D_>), grid, dim3(256), 0, s, x, ldx, y, ldy, res, ldres, sh, stats, gamma, beta, rng)
 #define CY_GNA_ACT(A_)             \
     do {                           \
         if (rng.q) CY_GNA(A_, true); \
         else CY_GNA(A_, false);    \
     } while (0)
-    if constexpr (V == 1) CY_GNA_ACT(-1);
-    else if (act == CY_ACT_MISH) CY_GNA_ACT(CY_ACT_MISH);
+    if (act == CY_ACT_MISH) CY_GNA_ACT(CY_ACT_MISH);
     else if (act == CY_ACT_LEAKY) CY_GNA_ACT(CY_ACT_LEAKY);
     else CY_GNA_ACT(CY_ACT_LINEAR);
 #undef CY_GNA_ACT
@@ -450,26 +470,106 @@ int backward(const T* x, int ldx, const T* dy, int lddy, T* dx, int lddx, T* res
 #define CY_GNB(A_, D_)                                                                                                        \
     do {                                                                                                                      \
         hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, A_, D_>), grid, dim3(256), 0, s, x, ldx, dy, lddy, sh, stats, gamma, beta, \
-                           act, rng, part);                                                                                   \
+                           rng, part);                                                                                   \
         CY_LAUNCH_CHECK();                                                                                                    \
         hipLaunchKernelGGL(gn_bwd_fold_kernel, fgrid, dim3(256), 0, s, part, sh, gamma, chan, s12);                            \
         CY_LAUNCH_CHECK();                                                                                                    \
         hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, A_, D_>), grid, dim3(256), 0, s, x, ldx, dy, lddy, dx, lddx, resg, ldrg, \
-                           res_accum, sh, stats, gamma, beta, chan, s12, ggamma, gbeta, gscale, accumulate, act, rng);         \
+                           res_accum, sh, stats, gamma, beta, chan, s12, ggamma, gbeta, gscale, accumulate, rng);              \
     } while (0)
 #define CY_GNB_ACT(A_)             \
     do {                           \
         if (rng.q) CY_GNB(A_, true); \
         else CY_GNB(A_, false);    \
     } while (0)
-    if constexpr (V == 1) CY_GNB_ACT(-1);
-    else if (act == CY_ACT_MISH) CY_GNB_ACT(CY_ACT_MISH);
+    if (act == CY_ACT_MISH) CY_GNB_ACT(CY_ACT_MISH);
     else if (act == CY_ACT_LEAKY) CY_GNB_ACT(CY_ACT_LEAKY);
     else CY_GNB_ACT(CY_ACT_LINEAR);
 #undef CY_GNB_ACT
 #undef CY_GNB
     CY_LAUNCH_CHECK();
     return 0;
+}
+
+// ---- the one-launch kernels: which calls take them ---------------------------------------------------------------------------
+// Test / tool switch (cy_gn_config)
+struct Config {
+    int mode, polls, width, R;
+};
+constexpr int POLLS = 1024;      // about a millisecond
+Config g_cfg = {1, POLLS, 0, 0};
+
+int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+// One shape of blocks: `width` 16-byte columns, R chunks to a thread.  false: its blocks cannot meet.
+bool plan_width(int N, long HW, int C, int G, int V, int width, int R, int polls, ResPlan& p) {
+    const int Cg = C / G, gps = width * V / Cg;
+    p.R = R;
+    p.sh = ResShape{HW, N, C, G, Cg, width, C / V / width, gps, GN_TB / width, 0, 0, 0, polls};
+    const long nb = (HW + (long)R * p.sh.rows - 1) / ((long)R * p.sh.rows), clusters = (long)N * p.sh.nspan;
+    if (nb > 512 || clusters * nb >= MAX_BLOCKS) return false;      // (half of the blocks that fit on the chip)
+    p.sh.nb = (int)nb;
+    if (nb > 1) {
+        if (nb * gps > GN_ONE_STEP) {      // two steps of about the same number of entries
+            int sub = 1;
+            while ((long)sub * sub < nb) ++sub;
+            p.sh.sub = sub;
+            p.sh.nsub = (int)((nb + sub - 1) / sub);
+        }
+        if (clusters > GN_MAX_CLUSTERS || clusters * (nb + p.sh.nsub) * gps > GN_MAX_PAIRS) return false;
+    }
+    return true;
+}
+
+// Columns of a block: the number nearest to eight (one 128-byte line a pixel) that cuts the row into equal spans of whole groups: narrow
+// spans make small clusters, and a narrower one splits cache lines.  16 x 76 x 76 x 256 f16 forward: 4 columns 29.2 us, 8: 24.8, 16: 24.7,
+// 32: 25.6; backward 52.9, 44.2, 44.0, 49.0; 16 x 38 x 38 x 512 f16 backward with 64: 30.8, 8: 26.9.
+// Chunks of a thread: 16 (backward 8: x and the 32-bit dz), half of that where fewer than 512 blocks would be left for 256 compute units:
+// 16 x 38 x 38 x 512 f16 forward (384 blocks at 16) 19.0 us with 16, 16.5 with 8; 16 x 76 x 76 x 256 f16 (768) 24.8 with 16, 28.8 with 8.
+bool plan_resident(int N, long HW, int C, int G, int V, bool bwd, ResPlan& p) {
+    const Config cfg = g_cfg;
+    if (!cfg.mode || C % V) return false;
+    const int Cg = C / G, unit = Cg / gcd(Cg, V);      // columns of the smallest span of whole groups and whole chunks
+    const int cpr = C / V, units = cpr / unit, most = bwd ? 8 : 16;
+    int tried = 0;      // (columns already looked at, as a lower bound of the distance from eight)
+    for (;;) {
+        int width = 0, best = 0;
+        for (int i = 1; i <= units && i * unit <= GN_TB; ++i) {
+            if (units % i) continue;
+            const int w = i * unit, far = w >= 8 ? w * 8 : 8 * 8 * 8 / w;      // 64 times the factor between w and 8
+            if (far * 2 + (w < 8) > tried && (!width || far * 2 + (w < 8) < best)) {
+                width = w;
+                best = far * 2 + (w < 8);
+            }
+        }
+        if (!width) return false;
+        tried = best;
+        if (cfg.width && cfg.width % unit == 0 && cpr % cfg.width == 0 && cfg.width <= GN_TB) width = cfg.width;
+        int R = cfg.R ? cfg.R * most / 16 : most;
+        if (!cfg.R) {
+            const long ppb = (long)most * (GN_TB / width);
+            if ((long)N * (cpr / width) * ((HW + ppb - 1) / ppb) < 512) R = most / 2;
+        }
+        if (plan_width(N, HW, C, G, V, width, R, cfg.polls, p)) return true;
+        if (cfg.width) return false;
+    }
+}
+
+// bytes behind the part of a workspace that stays zero
+int64_t resident_bytes(const ResPlan& p) {
+    const int64_t clusters = (int64_t)p.sh.N * p.sh.nspan;
+    return 8 * clusters * p.sh.gps + 8 * (int64_t)p.sh.N * p.sh.nb * p.sh.C + 4 * clusters * p.sh.nb;
+}
+
+ResWork resident_work(const ResPlan& p, char* ws) {
+    const int64_t clusters = (int64_t)p.sh.N * p.sh.nspan;
+    ResWork w;
+    w.counters = (unsigned*)ws;
+    w.pairs = (unsigned long long*)(ws + GN_COUNTER_BYTES);
+    w.fin = (unsigned long long*)(ws + GN_ZERO_BYTES);
+    w.chan = (float*)(w.fin + clusters * p.sh.gps);
+    w.list = (unsigned*)(w.chan + 2 * (int64_t)p.sh.N * p.sh.nb * p.sh.C);
+    return w;
 }
 
 // 16-byte accesses where every row of every operand starts on one
@@ -480,46 +580,69 @@ bool rows16(const void* p, int ld) {
 
 template <typename T>
 int forward_any(const void* x, int ldx, void* y, int ldy, const void* res, int ldres, int N, long HW, int C, int G,
-                const float* gamma, const float* beta, float eps, int act, const DropRng& rng, float* stats, float* ws,
+                const float* gamma, const float* beta, float eps, int act, const DropRng& rng, float* stats, char* ws,
                 int64_t ws_bytes, hipStream_t s) {
     constexpr int CH = Elem<T>::CH;
     if (!aligned_to(x, sizeof(T)) || !aligned_to(y, sizeof(T)) || !aligned_to(res, sizeof(T))) return CY_ERR_ARG;
     const bool vec = C % CH == 0 && rows16<T>(x, ldx) && rows16<T>(y, ldy) && rows16<T>(res, ldres);
+    ResPlan rp;
+    if (vec && plan_resident(N, HW, C, G, CH, false, rp)) {
+        if (ws_bytes < GN_ZERO_BYTES + resident_bytes(rp)) return CY_ERR_ARG;
+        return gn_resident_fwd(rp, ResFwd{x, ldx, y, ldy, res, ldres, gamma, beta, eps, stats}, resident_work(rp, ws), act, Elem<T>::DT, rng, s);
+    }
     const Shape sh = make_shape(N, HW, C, G, vec ? CH : 1);
-    if (ws_bytes < 4 * need_floats(sh)) return CY_ERR_ARG;
-    if (vec) return forward<T, CH>((const T*)x, ldx, (T*)y, ldy, (const T*)res, ldres, sh, gamma, beta, eps, act, rng, stats, ws, s);
-    return forward<T, 1>((const T*)x, ldx, (T*)y, ldy, (const T*)res, ldres, sh, gamma, beta, eps, act, rng, stats, ws, s);
+    if (ws_bytes < GN_ZERO_BYTES + 4 * need_floats(sh)) return CY_ERR_ARG;
+    float* fws = (float*)(ws + GN_ZERO_BYTES);
+    if (vec) return forward<T, CH>((const T*)x, ldx, (T*)y, ldy, (const T*)res, ldres, sh, gamma, beta, eps, act, rng, stats, fws, s);
+    return forward<T, 1>((const T*)x, ldx, (T*)y, ldy, (const T*)res, ldres, sh, gamma, beta, eps, act, rng, stats, fws, s);
 }
 
 template <typename T>
 int backward_any(const void* x, int ldx, const void* dy, int lddy, void* dx, int lddx, void* resg, int ldrg, int res_accum, int N,
                  long HW, int C, int G, const float* gamma, const float* beta, const float* stats, int act, const DropRng& rng,
-                 float* ggamma, float* gbeta, float gscale, int accumulate, float* ws, int64_t ws_bytes, hipStream_t s) {
+                 float* ggamma, float* gbeta, float gscale, int accumulate, char* ws, int64_t ws_bytes, hipStream_t s) {
     constexpr int CH = Elem<T>::CH;
     if (!aligned_to(x, sizeof(T)) || !aligned_to(dy, sizeof(T)) || !aligned_to(dx, sizeof(T)) || !aligned_to(resg, sizeof(T)))
         return CY_ERR_ARG;
     const bool vec = C % CH == 0 && rows16<T>(x, ldx) && rows16<T>(dy, lddy) && rows16<T>(dx, lddx) && rows16<T>(resg, ldrg);
+    ResPlan rp;
+    if (vec && plan_resident(N, HW, C, G, CH, true, rp)) {
+        if (ws_bytes < GN_ZERO_BYTES + resident_bytes(rp)) return CY_ERR_ARG;
+        return gn_resident_bwd(rp, ResBwd{x, ldx, dy, lddy, dx, lddx, resg, ldrg, res_accum, gamma, beta, stats, ggamma, gbeta, gscale, accumulate},
+                               resident_work(rp, ws), act, Elem<T>::DT, rng, s);
+    }
     const Shape sh = make_shape(N, HW, C, G, vec ? CH : 1);
-    if (ws_bytes < 4 * need_floats(sh)) return CY_ERR_ARG;
+    if (ws_bytes < GN_ZERO_BYTES + 4 * need_floats(sh)) return CY_ERR_ARG;
+    float* fws = (float*)(ws + GN_ZERO_BYTES);
     if (vec)
         return backward<T, CH>((const T*)x, ldx, (const T*)dy, lddy, (T*)dx, lddx, (T*)resg, ldrg, res_accum, sh, gamma, beta, stats,
-                               act, rng, ggamma, gbeta, gscale, accumulate, ws, s);
+                               act, rng, ggamma, gbeta, gscale, accumulate, fws, s);
     return backward<T, 1>((const T*)x, ldx, (const T*)dy, lddy, (T*)dx, lddx, (T*)resg, ldrg, res_accum, sh, gamma, beta, stats, act,
-                          rng, ggamma, gbeta, gscale, accumulate, ws, s);
+                          rng, ggamma, gbeta, gscale, accumulate, fws, s);
 }
 
 }  // namespace
 
 extern "C" int64_t cy_gn_workspace(int N, int64_t HW, int C, int groups, int dtype) {
     if (!sizes_ok(N, HW, C, groups, dtype)) return CY_ERR_ARG;
-    if (N == 0 || HW == 0) return 16;
-    int64_t most = need_floats(make_shape(N, (long)HW, C, groups, 1));       // (whichever access width a call's pointers allow)
+    if (N == 0 || HW == 0) return GN_ZERO_BYTES;
+    int64_t most = 4 * need_floats(make_shape(N, (long)HW, C, groups, 1));      // (whichever kernels a call's pointers allow)
     const int ch = dtype == CY_F32 ? 4 : 8;
     if (C % ch == 0) {
-        const int64_t v = need_floats(make_shape(N, (long)HW, C, groups, ch));
+        const int64_t v = 4 * need_floats(make_shape(N, (long)HW, C, groups, ch));
         if (v > most) most = v;
+        for (int bwd = 0; bwd < 2; ++bwd) {
+            ResPlan p;
+            if (plan_resident(N, (long)HW, C, groups, ch, bwd != 0, p) && resident_bytes(p) > most) most = resident_bytes(p);
+        }
     }
-    return 4 * most;
+    return GN_ZERO_BYTES + most;
+}
+
+extern "C" int cy_gn_config(int mode, int polls, int width, int chunks) {
+    if (mode < 0 || mode > 1 || polls < -1 || width < 0 || (chunks != 0 && chunks != 8 && chunks != 16)) return CY_ERR_ARG;
+    g_cfg = Config{mode, polls < 0 ? POLLS : polls, width, chunks};
+    return 0;
 }
 
 extern "C" int cy_gn_act_fwd(const void* x, int ldx, void* y, int ldy, const void* res, int ldres, int N, int64_t HW, int C,
@@ -533,7 +656,7 @@ extern "C" int cy_gn_act_fwd(const void* x, int ldx, void* y, int ldy, const voi
     if (N == 0 || HW == 0) return 0;
     if (!x || !y || !ws || !aligned_to(ws, 8) || !aligned_to(stats, 8)) return CY_ERR_ARG;
 #define CY_GNF(T) \
-    return forward_any<T>(x, ldx, y, ldy, res, ldres, N, (long)HW, C, groups, gamma, beta, eps, act, r, stats, (float*)ws, ws_bytes, cy_s(s))
+    return forward_any<T>(x, ldx, y, ldy, res, ldres, N, (long)HW, C, groups, gamma, beta, eps, act, r, stats, (char*)ws, ws_bytes, cy_s(s))
     if (dtype == CY_F16) CY_GNF(f16);
     if (dtype == CY_BF16) CY_GNF(bf16);
     CY_GNF(float);
@@ -558,7 +681,7 @@ extern "C" int cy_gn_act_bwd(const void* x, int ldx, const void* dy, int lddy, v
     if (!x || !dy || !dx || !stats || !ws || !aligned_to(ws, 8) || !aligned_to(stats, 8)) return CY_ERR_ARG;
 #define CY_GNBW(T)                                                                                                             \
     return backward_any<T>(x, ldx, dy, lddy, dx, lddx, res_grad, ldrg, res_accum, N, (long)HW, C, groups, gamma, beta, stats, act, r, \
-                           ggamma, gbeta, gscale, accumulate, (float*)ws, ws_bytes, cy_s(s))
+                           ggamma, gbeta, gscale, accumulate, (char*)ws, ws_bytes, cy_s(s))
     if (dtype == CY_F16) CY_GNBW(f16);
     if (dtype == CY_BF16) CY_GNBW(bf16);
     CY_GNBW(float);

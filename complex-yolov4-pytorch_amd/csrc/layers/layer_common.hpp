@@ -14,6 +14,20 @@ __device__ __forceinline__ void store_v(T* p, const float* f) {
     else *reinterpret_cast<u32x4*>(p) = f32_to_chunk<T>(f);
 }
 
+// the same in two steps, so that several loads can be in flight before the first is looked at
+template <typename T, int V>
+struct Raw {
+    u32x4 v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const u32x4*>(p); }
+    __device__ __forceinline__ void get(float* f) const { chunk_to_f32<T>(v, f); }
+};
+template <typename T>
+struct Raw<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ void get(float* f) const { f[0] = (float)v; }
+};
+
 // ---- dropout generator ---------------------------------------------------------------------------------------------------
 // Philox-4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011): a 128-bit counter goes
 // through ten rounds of two 32 x 32 -> 64 bit products under a 64-bit key.  Here key = seed, counter = (block, step, layer id):

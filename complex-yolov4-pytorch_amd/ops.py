@@ -607,11 +607,16 @@ def _drop_args(who, p, rng):
 
 
 def gn_workspace(N, H, W, C, groups, dt, device='cuda'):
-    """Scratch of gn_act_fwd / gn_act_bwd for one shape (contents arbitrary; one per stream that may run them at the same time)."""
+    """Zeroed scratch of gn_act_fwd / gn_act_bwd for one shape, theirs alone (one per stream that may run them at the same time)."""
     n = int(lib().raw('cy_gn_workspace')(N, H * W, C, groups, dt))
     if n < 0:
         raise CyoloError('cy_gn_workspace: %d channels in %d groups (N %d, %d x %d, type %r)' % (C, groups, N, H, W, dt))
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def gn_config(mode=1, polls=-1, width=0, chunks=0):
+    """Test / tool switch of the group norm kernels (cy_gn_config)."""
+    lib().call('cy_gn_config', int(mode), int(polls), int(width), int(chunks))
 
 
 def _check_gn(who, x, views, gamma, beta, stats, groups, act, ws, more=(), rng=None):

@@ -325,9 +325,9 @@ int cy_bn_act_bwd_apply(const void* x, int ldx, const void* dy, int lddy, void* 
  * (rows that all start on 16 bytes take the fast kernels).  y may be x (every element is read before it is written by the same
  * thread); no other overlap.  N = 0 or HW = 0: nothing to do.
  * Dropout (see cy_dropout): q > 0 drops with probability q / 65536, rng / id as there; element index = ((n * HW + pixel) * C + c).
- * ws: cy_gn_workspace() bytes, 8-byte aligned, contents arbitrary; used by the call from its first to its last launch (calls on
- * different streams, captured graphs that may run at the same time among them, need one each).
- * No atomics: results are bit-identical from run to run. */
+ * ws: cy_gn_workspace() bytes, 8-byte aligned, ZEROED ONCE by the caller; calls of any shape may share one that is large enough for
+ * each, one after the other (calls that may run at the same time -- other streams, captured graphs among them -- need one each).
+ * Results are bit-identical from run to run. */
 int cy_gn_act_fwd(const void* x, int ldx, void* y, int ldy, const void* res, int ldres, int N, int64_t HW, int C, int groups,
                   const float* gamma, const float* beta, float eps, int act, int dtype, float* stats, int q, const int64_t* rng,
                   int id, void* ws, int64_t ws_bytes, cy_stream_t s);
@@ -340,6 +340,11 @@ int cy_gn_act_bwd(const void* x, int ldx, const void* dy, int lddy, void* dx, in
                   void* ws, int64_t ws_bytes, cy_stream_t s);
 /* Bytes of ws for either call. */
 int64_t cy_gn_workspace(int N, int64_t HW, int C, int groups, int dtype);
+/* Test / tool switch, not used on the step path.  mode 0: the three-launch kernels always, 1: default (one launch where an image's rows
+ * start on 16 bytes and its blocks can meet); polls: how often a block of the one-launch kernels looks for the others before it leaves
+ * its pixels to the last of them (-1: default; 0: never waits); width / chunks > 0: 16-byte columns of a block / held by a thread where
+ * the shape allows (0: own policy).  A workspace is sized for the setting it was asked under. */
+int cy_gn_config(int mode, int polls, int width, int chunks);
 
 /* Dropout over a view of M pixels x C channels, the mask never stored:
  *   y = keep[e] ? x * 65536 / (65536 - q) : 0     (accumulate: added to what y holds)

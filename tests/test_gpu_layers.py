@@ -54,8 +54,24 @@ class Strided:
 
 def _workspace(N, H, W, C, G, dt):
     ws = ops.gn_workspace(N, H, W, C, G, dt)
-    ws.fill_(0xFF)      # (contents arbitrary: NaN in every type)
+    assert int(ws[:COUNTERS].max()) == 0
+    ws[COUNTERS:].fill_(0xFF)      # (behind the counters the contents are arbitrary: NaN in every type)
     return ws
+
+
+COUNTERS = 512 * 17 * 128 + 384 * 1024 * 8
+
+# the three-launch kernels; one launch by the library's own rule, with few and many blocks to an image, and with blocks that never wait
+# for the others (the last of an image's blocks then finishes all of them)
+KERNELS = {'general': dict(mode=0), 'policy': {}, 'chunks8': dict(chunks=8), 'chunks16': dict(chunks=16), 'nowait': dict(polls=0, chunks=8)}
+
+
+@pytest.fixture(params=list(KERNELS))
+def kernels(request):
+    kw = dict(KERNELS[request.param])
+    ops.gn_config(**kw)
+    yield request.param
+    ops.gn_config()
 
 
 def _stored(exact, dt):
@@ -85,6 +101,8 @@ SHAPES = [
     (2, 6, 6, 2056, 8, 0, 0),          # more columns than a block has threads (16-bit: 257)
     (1, 3, 3, 1030, 2, 0, 0),          # the same, one element at a time
     (40, 2, 3, 32, 32, 0, 0),          # a group per channel
+    (2, 50, 45, 64, 4, 0, 0),          # several blocks to an image in every kernel
+    (1, 160, 150, 64, 32, 0, 0),       # many blocks and many groups: they meet in two steps
     (2, 100, 90, 32, 8, 0, 0),         # several pixel ranges per image
     (1, 1, 1, 1, 1, 0, 0),
 ]
@@ -113,7 +131,7 @@ def _stats_tol(x, G):
 @pytest.mark.parametrize('act', [0, 1, 2], ids=['linear', 'leaky', 'mish'])
 @pytest.mark.parametrize('dt', [CY_F16, CY_BF16, CY_F32], ids=['f16', 'bf16', 'f32'])
 @pytest.mark.parametrize('shape', SHAPES, ids=IDS)
-def test_group_norm_act(shape, dt, act, drop):
+def test_group_norm_act(shape, dt, act, drop, kernels):
     N, H, W, C, G, pad, off = shape
     x, dy, res, gamma, beta = _problem(shape, dt, 100 + C)
     use_res = act != 1
@@ -185,12 +203,13 @@ def test_group_norm_act(shape, dt, act, drop):
     gg3 = torch.full((2, C), float('nan'), device=DEV)
     ops.gn_act_bwd(xs.view, dys.view, dxs.view, None, False, ga, be, stats, G, act, None, gg3[1], 1.0, False, ws, drop, rng, LAYER)
     assert torch.equal(gg3[1], gg2[1]) and bool(gg3[0].isnan().all())
+    assert int(ws[:COUNTERS].max()) == 0      # (as it was: the next call finds its counters)
     _close(gg2.cpu().double() * 0.5 + g0.double(), got, 4 * E * (got.abs() + g0.double().abs()), 'stored gradients')
 
 
 @pytest.mark.parametrize('dt', [CY_F16, CY_BF16, CY_F32], ids=['f16', 'bf16', 'f32'])
 @pytest.mark.parametrize('shape', [(2, 40, 41, 64, 8, 0, 0), (1, 50, 50, 30, 5, 0, 0)], ids=['rows16', 'ragged'])
-def test_statistics_beside_a_large_mean(shape, dt):
+def test_statistics_beside_a_large_mean(shape, dt, kernels):
     """Deviations of a step or two of the type beside the mean: sums of squares of the values would lose them all."""
     N, H, W, C, G, pad, off = shape
     g = _gen(5)
