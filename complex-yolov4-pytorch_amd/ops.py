@@ -558,27 +558,61 @@ def bn_act_bwd_apply(x, dy, dx, res_grad, res_accum, mean, invstd, scale, shift,
 
 # ---- per-image layers: group norm + activation, dropout ---------------------------------------------
 
-def _check_layer(who, first, views=(), floats=(), rng=None):
-    """Arguments of the per-image layers: views of one shape, type and device, float32 vectors of given sizes on that device, and
-    that device the current one (the launch goes to its current stream)."""
+# (A layer call on a small map is shorter on the GPU than in this file: pointers travel as plain integers, each argument is looked at
+# once, and the stream is asked for through torch's raw-handle query.  15 -> 7 us of host time a call.)
+
+def _layer_device(who, first):
+    """The index of the device the call runs on: that of its first view, which has to be the current one (the launch goes to its
+    current stream)."""
     _require_gpu()
-    dev = first.buf.device
-    check_device_tensor(first.buf, who)
-    if dev.index != torch.cuda.current_device():
-        raise CyoloError('%s: the tensors are on %s, the current device is cuda:%d' % (who, dev, torch.cuda.current_device()))
-    dt = _TORCH_DT.get(first.dt)
-    for v in (first,) + tuple(views):
-        if v is None:
-            continue
-        if (v.N, v.H, v.W, v.C, v.dt) != (first.N, first.H, first.W, first.C, first.dt) or v.buf.dtype != dt or v.buf.device != dev:
-            raise CyoloError('%s: views differ in shape, type or device: %s and %s' % (who, _view_str(first), _view_str(v)))
-        if v.ld < v.C or v.off < 0 or (v.M and v.off + (v.M - 1) * v.ld + v.C > v.buf.numel()) or not v.buf.is_contiguous():
-            raise CyoloError('%s: %s reaches beyond its buffer of %d elements' % (who, _view_str(v), v.buf.numel()))
-    for name, t, n in floats:
-        if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.device != dev or not t.is_contiguous()):
-            raise CyoloError('%s: %s must be %d contiguous float32 values on %s' % (who, name, n, dev))
-    if rng is not None and (rng.dtype != torch.int64 or rng.numel() != 2 or rng.device != dev or not rng.is_contiguous()):
-        raise CyoloError('%s: the generator state is a contiguous int64 tensor (seed, step) on %s (ops.dropout_state)' % (who, dev))
+    buf = first.buf
+    dev = buf.get_device()
+    if dev != torch.cuda.current_device():
+        check_device_tensor(buf, who)
+        raise CyoloError('%s: the tensors are on %s, the current device is cuda:%d' % (who, buf.device, torch.cuda.current_device()))
+    if buf.dtype is not _TORCH_DT.get(first.dt):
+        raise CyoloError('%s: %s of type %r' % (who, _view_str(first), first.dt))
+    return dev
+
+
+def _layer_view(who, v, first, dev):
+    """Address of a view of ``first``'s shape, type and device that lies inside its buffer (None: None)."""
+    if v is None:
+        return None
+    buf = v.buf
+    if (v.C != first.C or v.W != first.W or v.H != first.H or v.N != first.N or v.dt != first.dt or buf.dtype is not first.buf.dtype
+            or buf.get_device() != dev):
+        raise CyoloError('%s: views differ in shape, type or device: %s and %s' % (who, _view_str(first), _view_str(v)))
+    m = v.N * v.H * v.W
+    if v.ld < v.C or v.off < 0 or (m and v.off + (m - 1) * v.ld + v.C > buf.numel()) or not buf.is_contiguous():
+        raise CyoloError('%s: %s reaches beyond its buffer of %d elements' % (who, _view_str(v), buf.numel()))
+    return buf.data_ptr() + v.off * _ELSIZE[v.dt]
+
+
+def _layer_floats(who, name, t, n, dev):
+    """Address of n contiguous float32 values (None: None)."""
+    if t is None:
+        return None
+    if t.dtype is not torch.float32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise CyoloError('%s: %s must be %d contiguous float32 values on the views\' device' % (who, name, n))
+    return t.data_ptr()
+
+
+def _layer_drop(who, p, rng, dev):
+    """-> (65536ths, address of the generator state)."""
+    q = dropout_q(p)
+    if rng is None:
+        if q:
+            raise CyoloError('%s: dropout needs the generator state (ops.dropout_state)' % who)
+        return 0, None
+    if rng.dtype is not torch.int64 or rng.numel() != 2 or rng.get_device() != dev or not rng.is_contiguous():
+        raise CyoloError('%s: the generator state is a contiguous int64 tensor (seed, step) on the views\' device (ops.dropout_state)' % who)
+    return q, rng.data_ptr()
+
+
+def _layer_stream(dev):
+    h = getattr(_TLS, 'handle', None)
+    return h if h is not None else torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _view_str(v):
@@ -599,19 +633,17 @@ def dropout_state(seed, device='cuda', step=0):
     return torch.tensor([seed - (1 << 64) if seed >> 63 else seed, int(step)], dtype=torch.int64, device=device)
 
 
-def _drop_args(who, p, rng):
-    q = dropout_q(p)
-    if q and rng is None:
-        raise CyoloError('%s: dropout needs the generator state (ops.dropout_state)' % who)
-    return q
+def gn_workspace_bytes(N, H, W, C, groups, dt):
+    """Size of the workspace of gn_act_fwd / gn_act_bwd for one shape; a larger one does as well."""
+    n = int(lib().raw('cy_gn_workspace')(N, H * W, C, groups, dt))
+    if n < 0:
+        raise CyoloError('cy_gn_workspace: %d channels in %d groups (N %d, %d x %d, type %r)' % (C, groups, N, H, W, dt))
+    return n
 
 
 def gn_workspace(N, H, W, C, groups, dt, device='cuda'):
     """Zeroed scratch of gn_act_fwd / gn_act_bwd for one shape, theirs alone (one per stream that may run them at the same time)."""
-    n = int(lib().raw('cy_gn_workspace')(N, H * W, C, groups, dt))
-    if n < 0:
-        raise CyoloError('cy_gn_workspace: %d channels in %d groups (N %d, %d x %d, type %r)' % (C, groups, N, H, W, dt))
-    return torch.zeros(n, dtype=torch.uint8, device=device)
+    return torch.zeros(gn_workspace_bytes(N, H, W, C, groups, dt), dtype=torch.uint8, device=device)
 
 
 def gn_config(mode=1, polls=-1, width=0, chunks=0):
@@ -619,59 +651,65 @@ def gn_config(mode=1, polls=-1, width=0, chunks=0):
     lib().call('cy_gn_config', int(mode), int(polls), int(width), int(chunks))
 
 
-def _check_gn(who, x, views, gamma, beta, stats, groups, act, ws, more=(), rng=None):
+def _check_gn(who, x, gamma, beta, groups, act, ws, dev):
     if groups < 1 or x.C % groups:
         raise CyoloError('%s: %d channels do not divide into %d groups' % (who, x.C, groups))
     if act not in (0, 1, 2):
         raise CyoloError('%s: unsupported activation %r' % (who, act))
     if gamma is None or beta is None:
         raise CyoloError('%s: scale and shift are needed' % who)
-    _check_layer(who, x, views, (('gamma', gamma, x.C), ('beta', beta, x.C), ('stats', stats, 2 * x.N * groups)) + more, rng)
-    if ws is None or ws.device != x.buf.device or not ws.is_contiguous():
-        raise CyoloError('%s: the workspace is a contiguous tensor on %s (ops.gn_workspace)' % (who, x.buf.device))
+    if ws is None or ws.get_device() != dev or not ws.is_contiguous():
+        raise CyoloError('%s: the workspace is a contiguous tensor on the views\' device (ops.gn_workspace)' % who)
 
 
 def gn_act_fwd(x, y, res, gamma, beta, groups, eps, act, stats, ws, drop=0.0, rng=None, drop_id=0):
     """y = res + dropout(act(group norm of x)); stats: float32 [N, groups, 2] (mean, 1 / deviation) for gn_act_bwd, or None."""
-    _check_gn('gn_act_fwd', x, (y, res), gamma, beta, stats, groups, act, ws, rng=rng)
-    if not eps >= 0.0:
-        raise CyoloError('gn_act_fwd: eps %r' % eps)
-    q = _drop_args('gn_act_fwd', drop, rng)
-    lib().call('cy_gn_act_fwd', _p(x), x.ld, _p(y), y.ld, _p(res), res.ld if res is not None else 0, x.N, x.H * x.W, x.C, groups, _p(gamma),
-               _p(beta), float(eps), act, x.dt, _p(stats), q, _p(rng), int(drop_id), _p(ws), ws.numel() * ws.element_size(),
-               _stream())
+    who = 'gn_act_fwd'
+    dev = _layer_device(who, x)
+    _check_gn(who, x, gamma, beta, groups, act, ws, dev)
+    if y is None or not eps >= 0.0:
+        raise CyoloError('gn_act_fwd: an output and eps >= 0 are needed')
+    q, state = _layer_drop(who, drop, rng, dev)
+    lib().call('cy_gn_act_fwd', _layer_view(who, x, x, dev), x.ld, _layer_view(who, y, x, dev), y.ld, _layer_view(who, res, x, dev),
+               res.ld if res is not None else 0, x.N, x.H * x.W, x.C, groups, _layer_floats(who, 'gamma', gamma, x.C, dev),
+               _layer_floats(who, 'beta', beta, x.C, dev), eps, act, x.dt, _layer_floats(who, 'stats', stats, 2 * x.N * groups, dev), q,
+               state, drop_id, ws.data_ptr(), ws.numel() * ws.element_size(), _layer_stream(dev))
 
 
 def gn_act_bwd(x, dy, dx, res_grad, res_accum, gamma, beta, stats, groups, act, ggamma, gbeta, gscale, accumulate, ws, drop=0.0, rng=None,
                drop_id=0):
     """dx (may be dy), ggamma / gbeta (+)= gscale * sums (None: not wanted); res_grad (+)= dy, the shortcut branch's gradient."""
-    if stats is None:
-        raise CyoloError('gn_act_bwd: the statistics of the forward pass are needed')
-    _check_gn('gn_act_bwd', x, (dy, dx, res_grad), gamma, beta, stats, groups, act, ws,
-              (('ggamma', ggamma, x.C), ('gbeta', gbeta, x.C)), rng)
-    q = _drop_args('gn_act_bwd', drop, rng)
-    lib().call('cy_gn_act_bwd', _p(x), x.ld, _p(dy), dy.ld, _p(dx), dx.ld, _p(res_grad), res_grad.ld if res_grad is not None else 0,
-               int(bool(res_accum)), x.N, x.H * x.W, x.C, groups, _p(gamma), _p(beta), _p(stats), act, x.dt, _p(ggamma), _p(gbeta),
-               float(gscale), int(bool(accumulate)), q, _p(rng), int(drop_id), _p(ws), ws.numel() * ws.element_size(), _stream())
+    who = 'gn_act_bwd'
+    dev = _layer_device(who, x)
+    _check_gn(who, x, gamma, beta, groups, act, ws, dev)
+    if dy is None or dx is None or stats is None:
+        raise CyoloError('gn_act_bwd: dy, dx and the statistics of the forward pass are needed')
+    q, state = _layer_drop(who, drop, rng, dev)
+    lib().call('cy_gn_act_bwd', _layer_view(who, x, x, dev), x.ld, _layer_view(who, dy, x, dev), dy.ld, _layer_view(who, dx, x, dev), dx.ld,
+               _layer_view(who, res_grad, x, dev), res_grad.ld if res_grad is not None else 0, 1 if res_accum else 0, x.N, x.H * x.W, x.C,
+               groups, _layer_floats(who, 'gamma', gamma, x.C, dev), _layer_floats(who, 'beta', beta, x.C, dev),
+               _layer_floats(who, 'stats', stats, 2 * x.N * groups, dev), act, x.dt, _layer_floats(who, 'ggamma', ggamma, x.C, dev),
+               _layer_floats(who, 'gbeta', gbeta, x.C, dev), gscale, 1 if accumulate else 0, q, state, drop_id, ws.data_ptr(),
+               ws.numel() * ws.element_size(), _layer_stream(dev))
 
 
 def dropout_fwd(x, y, p, rng, drop_id=0):
     """y = kept ? x / (1 - p) : 0 (y may be x); the mask is a function of (rng, drop_id, element index) and is never stored."""
-    _check_layer('dropout_fwd', x, (y,), rng=rng)
-    _dropout('dropout_fwd', x, y, p, rng, drop_id, False)
+    _dropout('dropout_fwd', x, y, p, rng, drop_id, 0)
 
 
 def dropout_bwd(dy, dx, accumulate, p, rng, drop_id=0):
     """dx (+)= the same map of dy."""
-    _check_layer('dropout_bwd', dy, (dx,), rng=rng)
-    _dropout('dropout_bwd', dy, dx, p, rng, drop_id, accumulate)
+    _dropout('dropout_bwd', dy, dx, p, rng, drop_id, 1 if accumulate else 0)
 
 
 def _dropout(who, x, y, p, rng, drop_id, accumulate):
-    if rng is None:
-        raise CyoloError('%s: dropout needs the generator state (ops.dropout_state)' % who)
-    q = dropout_q(p)
-    lib().call('cy_dropout', _p(x), x.ld, _p(y), y.ld, x.M, x.C, q, _p(rng), int(drop_id), int(bool(accumulate)), x.dt, _stream())
+    dev = _layer_device(who, x)
+    if rng is None or y is None:
+        raise CyoloError('%s: an output and the generator state (ops.dropout_state) are needed' % who)
+    q, state = _layer_drop(who, p, rng, dev)
+    lib().call('cy_dropout', _layer_view(who, x, x, dev), x.ld, _layer_view(who, y, x, dev), y.ld, x.N * x.H * x.W, x.C, q, state, drop_id,
+               accumulate, x.dt, _layer_stream(dev))
 
 
 def maxpool_argmax_bytes(N, H, OH, OW, C):

@@ -122,7 +122,7 @@ def on_cpu(monkeypatch):
     """The operator layer's checks with host tensors standing in for device tensors; a call that reaches the library fails the test."""
     monkeypatch.setattr(ops, '_require_gpu', lambda: None)
     monkeypatch.setattr(ops, 'check_device_tensor', lambda t, who: None)
-    monkeypatch.setattr(torch.cuda, 'current_device', lambda: None)      # torch.device('cpu').index
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: -1)      # what a host tensor's get_device() says
 
     class NoCalls:
         def call(self, name, *a):
