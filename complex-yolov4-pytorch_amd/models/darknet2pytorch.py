@@ -15,14 +15,17 @@ Differences from the reference that a caller can observe (all deliberate, SURVEY
     slices are the parameters' ``.grad`` (this is what the data-parallel wrapper all-reduces);
   * ``dtype='f16'`` (default) / ``'bf16'`` store activations and packed weights in 16 bits and accumulate in fp32
     (bf16 needs no loss scaling); ``dtype='f32'`` is the parity mode;
-  * ``deterministic=True`` replaces the fp32-atomic reductions by fixed-order ones: repeats are bit-identical.
+  * ``deterministic=True`` replaces the fp32-atomic reductions by fixed-order ones: repeats are bit-identical;
+  * two cfg features beyond the reference's: ``group_normalize=<groups>`` in a [convolutional] block (instead of batch_normalize:
+    statistics of one image, the same function in training and evaluation; parameters ``gn{n}.weight`` / ``.bias``) and the [dropout]
+    block (``probability``); its masks are a function of (``seed_dropout``'s seed, the count of training forwards, the module).
 """
 
 import torch
 import torch.nn as nn
 
 from .. import ops
-from .darknet_utils import load_conv, load_conv_bn, parse_cfg, print_cfg, save_conv, save_conv_bn
+from .darknet_utils import load_conv, load_conv_bn, load_conv_gn, parse_cfg, print_cfg, save_conv, save_conv_bn, save_conv_gn
 from .engine import Arena, Engine
 from .graph import Plan, lower_blocks
 from .yolo_layer import YoloLayer
@@ -55,7 +58,8 @@ class _StepFn(torch.autograd.Function):
     def forward(ctx, model, x, targets, *params):
         eng = model._engine_for(x)
         model._weights_epoch += 1            # a training step is under way: cached eval packs are stale from here on
-        outputs = eng.forward(x, targets, model._param_table(), model.use_giou_loss, x.shape[2])
+        outputs = eng.forward(x, targets, model._param_table(), model.use_giou_loss, x.shape[2],
+                              rng=model._dropout_state(x.device) if eng.rng is not None else None)
         model._publish_metrics(eng)
         heads = [m[0] for m in eng.metrics]
         total = heads[0].clone()
@@ -103,6 +107,7 @@ class Darknet(nn.Module):
         self.loss = self.models[len(self.models) - 1]
         self.header = torch.IntTensor([0, 0, 0, 0])
         self.seen = 0
+        self._drop_seed, self._drop_step, self._drop_dev = None, 0, None      # [dropout]: see seed_dropout
         self.cpu_outputs = True          # targets=None returns a CPU tensor like the reference (:228)
         import collections
         self._plans, self._engines = {}, collections.OrderedDict()      # engines in least-recently-used order (see _engine_for)
@@ -133,9 +138,11 @@ class Darknet(nn.Module):
             if t == 'convolutional':
                 n = m['n']
                 seq = nn.Sequential()
-                seq.add_module('conv%d' % n, nn.Conv2d(m['cin'], m['cout'], m['k'], m['stride'], m['pad'], bias=not m['bn']))
+                seq.add_module('conv%d' % n, nn.Conv2d(m['cin'], m['cout'], m['k'], m['stride'], m['pad'], bias=not m['norm']))
                 if m['bn']:
                     seq.add_module('bn%d' % n, nn.BatchNorm2d(m['cout']))
+                elif m['gn']:
+                    seq.add_module('gn%d' % n, nn.GroupNorm(m['gn'], m['cout']))
                 if m['act'] == 'leaky':
                     seq.add_module('leaky%d' % n, nn.LeakyReLU(0.1, inplace=True))
                 elif m['act'] == 'mish':
@@ -158,6 +165,31 @@ class Darknet(nn.Module):
         """Tell cached eval engines that parameters changed outside Darknet's sight (an in-place edit, an optimizer
         stepping without a training forward of this module).  Only needed with ``static_eval_weights = True``."""
         self._weights_epoch += 1
+
+    def seed_dropout(self, seed, step=0):
+        """Seed of the [dropout] masks (default: torch.initial_seed(), with the rank mixed in under torch.distributed: ranks that
+        share a seed would drop the same places of their different images) and the number of training forwards done so far:
+        ``seed_dropout(*model.dropout_position())`` after a resume continues the sequence."""
+        self._drop_seed, self._drop_step = int(seed), int(step)
+        if self._drop_dev is not None:      # (in place: a captured step reads and advances this tensor)
+            self._drop_dev.copy_(ops.dropout_state(seed, self._drop_dev.device, step))
+
+    def dropout_position(self):
+        """(seed, training forwards done) of the dropout masks; reads the device counter."""
+        if self._drop_dev is not None:
+            self._drop_step = int(self._drop_dev[1])
+        return self._drop_seed, self._drop_step
+
+    def _dropout_state(self, device):
+        if self._drop_dev is None or self._drop_dev.device != device:
+            seed, step = self.dropout_position()
+            if seed is None:
+                seed = torch.initial_seed()
+                if torch.distributed.is_available() and torch.distributed.is_initialized():
+                    seed += torch.distributed.get_rank() * 0x9E3779B97F4A7C15
+                self._drop_seed = seed = seed % (1 << 64)
+            self._drop_dev = ops.dropout_state(seed, device, step)
+        return self._drop_dev
 
     def load_state_dict(self, *args, **kwargs):
         self._weights_epoch += 1
@@ -188,6 +220,8 @@ class Darknet(nn.Module):
             model = self.models[ind]
             if int(block['batch_normalize']):
                 start = load_conv_bn(buf, start, model[0], model[1])
+            elif int(block.get('group_normalize', 0)):
+                start = load_conv_gn(buf, start, model[0], model[1])
             else:
                 start = load_conv(buf, start, model[0])
         return start
@@ -212,6 +246,8 @@ class Darknet(nn.Module):
                 model = self.models[ind]
                 if int(block['batch_normalize']):
                     save_conv_bn(fp, model[0], model[1])
+                elif int(block.get('group_normalize', 0)):
+                    save_conv_gn(fp, model[0], model[1])
                 else:
                     save_conv(fp, model[0])
 
@@ -325,7 +361,8 @@ class Darknet(nn.Module):
         if targets is None:
             eng = self._engine_for(x)
             out = eng.forward(x, None, self._param_table(), self.use_giou_loss, x.shape[2],
-                              weights_epoch=self._weights_epoch if self.static_eval_weights else None)
+                              weights_epoch=self._weights_epoch if self.static_eval_weights else None,
+                              rng=self._dropout_state(x.device) if eng.rng is not None else None)
             return out.cpu() if self.cpu_outputs else out.clone()
         targets = targets.to(x.device).float().contiguous()
         if self._plist is None:

@@ -8,7 +8,7 @@ load_conv_bn / load_conv / save_conv_bn / save_conv (reference :199-246).
 """
 import torch
 
-__all__ = ['parse_cfg', 'print_cfg', 'load_conv_bn', 'load_conv', 'save_conv_bn', 'save_conv']
+__all__ = ['parse_cfg', 'print_cfg', 'load_conv_bn', 'load_conv_gn', 'load_conv', 'save_conv_bn', 'save_conv_gn', 'save_conv']
 
 
 def parse_cfg(cfgfile):
@@ -69,6 +69,14 @@ def load_conv_bn(buf, start, conv_model, bn_model):
     return start
 
 
+def load_conv_gn(buf, start, conv_model, gn_model):
+    """A group-normalised block: the order of load_conv_bn without running statistics (gn.bias, gn.weight, conv.weight)."""
+    with torch.no_grad():
+        for t in (gn_model.bias.data, gn_model.weight.data, conv_model.weight.data):
+            start = _take(buf, start, t)
+    return start
+
+
 def load_conv(buf, start, conv_model):
     with torch.no_grad():
         start = _take(buf, start, conv_model.bias.data)
@@ -82,6 +90,11 @@ def _put(fp, t):
 
 def save_conv_bn(fp, conv_model, bn_model):
     for t in (bn_model.bias.data, bn_model.weight.data, bn_model.running_mean, bn_model.running_var, conv_model.weight.data):
+        _put(fp, t)
+
+
+def save_conv_gn(fp, conv_model, gn_model):
+    for t in (gn_model.bias.data, gn_model.weight.data, conv_model.weight.data):
         _put(fp, t)
 
 

@@ -15,6 +15,7 @@ from .. import ops, tune
 from ..ops import CONV_ACCUM, CONV_BIAS_F32OUT, CONV_STATS, CONV_TRANSPOSED, CY_F32, View
 
 BN_EPS, BN_MOMENTUM = 1e-5, 0.1          # torch.nn.BatchNorm2d defaults, as the reference uses them
+GN_EPS = 1e-5                            # torch.nn.GroupNorm's default
 
 
 def _pad32(c):
@@ -23,8 +24,8 @@ def _pad32(c):
 
 def _wgrad_rows(rec):
     """Rows of a weight-gradient slab = channels of the gradient view cy_conv_wgrad is handed: the real channel count of a
-    BatchNorm conv's output (complex_yolov3_tiny.cfg's first layer has 16), the 32-padded staging tensor of a head conv."""
-    return rec['cout'] if rec['bn'] else _pad32(rec['cout'])
+    normalised conv's output (complex_yolov3_tiny.cfg's first layer has 16), the 32-padded staging tensor of a head conv."""
+    return rec['cout'] if rec['norm'] else _pad32(rec['cout'])
 
 
 _PW_DIRECT = ((64, 64), (128, 64), (64, 128), (64, 32), (32, 64))    # (Cin, Cout) of the 1x1 streaming kernel (conv_direct.hip)
@@ -255,6 +256,16 @@ class Engine:
         self.dgs, self.dbs = new('dgs', max_c, torch.float32), new('dbs', max_c, torch.float32)
         # deterministic mode: second-stage table of the two-stage folds (<= 256 rows) / partial rows of the head bias gradient
         self.fold_tmp = new('fold_tmp', max(256 * 2 * max_c, 256 * 32), torch.float32, zero=True) if self.det else None
+        # group norm: (mean, 1 / deviation) per image and group for the backward pass; one workspace, the layers use it in turn
+        self.gnstats, gn_bytes = {}, 0
+        for rec in plan.convs:
+            if rec['gn']:
+                if training:
+                    self.gnstats[rec['idx']] = new('gnstats[%d]' % rec['idx'], (N, rec['gn'], 2), torch.float32)
+                gn_bytes = max(gn_bytes, ops.gn_workspace_bytes(N, rec['H'], rec['W'], rec['cout'], rec['gn'], dt))
+        self.gn_ws = new('gn workspace', gn_bytes, torch.uint8, zero=True) if gn_bytes else None
+        # dropout: (seed, step) of the pass under way -- a copy of the model's, so that a backward pass sees its own forward's
+        self.rng = new('dropout state', 2, torch.int64, zero=True) if training and plan.has_dropout else None
         # split-K slabs of every conv stay resident until their group is folded (table-driven, a few launches per step)
         self.wpart = new('wpart (split-K slabs)', max(max_wpart, 1), torch.float32)
         self._pack_table = self._pack_key = self._pack_epoch = None
@@ -430,10 +441,13 @@ class Engine:
             return ops.stream_scope(torch.cuda.current_stream(self.device))
         return contextlib.nullcontext()
 
-    def forward(self, x, targets, params, use_giou, img_size, weights_epoch=None):
+    def forward(self, x, targets, params, use_giou, img_size, weights_epoch=None, rng=None):
         plan = self.plan
         self.fwd_serial += 1
         self.passes += 1
+        if self.rng is not None:      # (outside the recorded list: the list reads the state from the engine's buffer)
+            rng[1:].add_(1)
+            self.rng.copy_(rng)
         self._pending_heads = []          # (a forward that raised after queueing a head must not leak it into this one)
         if self.stats_pair is not None and self.training:
             # the alternating statistics tables restart from a defined state every pass (complex_yolov4.cfg has an ODD number of
@@ -664,17 +678,30 @@ class Engine:
             nm = rec['_names'] = ('models.%d.conv%d' % (i, n), 'models.%d.bn%d' % (i, n))
         return nm
 
+    @staticmethod
+    def _gn_name(rec):
+        return 'models.%d.gn%d' % (rec['idx'], rec['n'])
+
     def _f_conv(self, rec, targets, use_giou, img_size):
         cname, bname = self._names(rec)
         P = self.params
         idx = rec['idx']
         cop = _pad32(rec['cout'])
         xv = self.view(rec['x'])
-        if not rec['bn']:
+        if not rec['norm']:
             ops.conv_igemm(xv, self.wf[idx], cop, self.view(rec['out']), rec['ks'], rec['stride'], rec['pad'],
                            flags=CONV_BIAS_F32OUT, bias=P[cname + '.bias'])
             return
         raw = self.view(rec['raw'])
+        if rec['gn']:
+            # the same in training and evaluation, but for the kept statistics and the dropout
+            with ops.prof('igemm', *self._conv_work(rec)):
+                ops.conv_igemm(xv, self.wf[idx], cop, raw, rec['ks'], rec['stride'], rec['pad'], tile=self._fwd_tile.get(idx, 0))
+            gname = self._gn_name(rec)
+            ops.gn_act_fwd(raw, self.view(rec['out']), self.view(rec['res']) if rec['res'] is not None else None, P[gname + '.weight'],
+                           P[gname + '.bias'], rec['gn'], GN_EPS, ops.ACT[rec['act']], self.gnstats.get(idx), self.gn_ws,
+                           rec['drop'] if self.training else 0.0, self.rng, rec['drop_id'])
+            return
         vec = self.bnvec[idx]
         mean, invstd, scale, shift = vec[0], vec[1], vec[2], vec[3]
         C, M = rec['cout'], raw.M
@@ -741,6 +768,12 @@ class Engine:
     def _f_pool(self, rec, *_):
         ops.maxpool_fwd(self.view(rec['x']), self.view(rec['out']), rec['k'], rec['stride'], rec['pad'],
                         self.argmax.get(rec['idx']), self.pool_scratch)
+
+    def _f_dropout(self, rec, *_):
+        if self.training and rec['p'] > 0:
+            ops.dropout_fwd(self.view(rec['x']), self.view(rec['out']), rec['p'], self.rng, rec['idx'])
+        else:
+            ops.slice_copy(self.view(rec['x']), self.view(rec['out']))
 
     def _f_upsample(self, rec, *_):
         ops.upsample_fwd(self.view(rec['x']), self.view(rec['out']), rec['stride'])
@@ -1101,10 +1134,16 @@ class Engine:
         if not self._tunable():
             return
         for rec in self.plan.convs:
-            if not rec['bn']:
+            if not rec['norm']:
                 continue
             idx, cop = rec['idx'], _pad32(rec['cout'])
             xv = self.view(rec['x'])
+            if rec['gn']:
+                raw = self.view(rec['raw'])
+                key = ('fwd plain', self.dt, xv.N, xv.H, xv.W, xv.C, xv.ld, raw.C, raw.ld, rec['ks'], rec['stride'])
+                self._fwd_tile[idx] = self._time_hints(key, lambda h: ops.conv_igemm(
+                    xv, self.wf[idx], cop, raw, rec['ks'], rec['stride'], rec['pad'], tile=h), xv.C, raw.C, ks=rec['ks'], slab=_slab_shape(rec))
+                continue
             pr, role = self._pair(idx)
             if role == 1:
                 continue                  # (convolved by its sibling's launch)
@@ -1362,8 +1401,31 @@ class Engine:
                                rec['pad'], flags=CONV_TRANSPOSED | (CONV_ACCUM if acc else 0),
                                tile=self._dgrad_tile.get((rec['idx'], ref.c0), 0))
 
+    def _b_gn_conv_bwd(self, b):
+        rec = b['fwd']
+        raw, g, gname = self.view(rec['raw']), self.view(rec['out'], grad=True), self._gn_name(rec)
+        res_view, res_acc = self._res_grad(b, g)
+        ops.gn_act_bwd(raw, g, g, res_view, res_acc, self.params[gname + '.weight'], self.params[gname + '.bias'], self.gnstats[rec['idx']],
+                       rec['gn'], ops.ACT[rec['act']], self.grads[gname + '.weight'], self.grads[gname + '.bias'], 1.0 / self.ls, True,
+                       self.gn_ws, rec['drop'], self.rng, rec['drop_id'])
+        self._wgrad(rec, g, self.view(rec['x']))
+        self._dgrad(rec, g, b['dx'])
+
+    def _res_grad(self, b, g):
+        """Where the normalisation pass puts the gradient of a folded shortcut's other branch: (view or None, accumulate)."""
+        runs = b['res_runs']
+        if len(runs) == 1:
+            return self.view(runs[0][0], grad=True), runs[0][1]
+        res = b['fwd']['res']
+        for ref, acc in runs:
+            ops.slice_copy(g.channels(ref.c0 - res.c0, ref.C), self.view(ref, grad=True), accumulate=acc)
+        return None, False
+
     def _b_conv_bwd(self, b):
         rec = b['fwd']
+        if rec['gn']:
+            self._b_gn_conv_bwd(b)
+            return
         idx = rec['idx']
         _, bname = self._names(rec)
         vec = self.bnvec[idx]
@@ -1390,14 +1452,8 @@ class Engine:
                 ftbl, frows = self.fold_tmp, ops.fold_rows(self.bnpart, rows, 2 * C, self.fold_tmp)
             ops.bn_bwd_finalize(ftbl, frows, C, self.dgs, self.dbs,
                                 self.grads[bname + '.weight'], self.grads[bname + '.bias'], 1.0 / self.ls)
-        res_view, res_acc = None, False
         runs = b['res_runs']
-        if len(runs) == 1:
-            res_view, res_acc = self.view(runs[0][0], grad=True), runs[0][1]
-        elif len(runs) > 1:
-            res = rec['res']
-            for ref, acc in runs:
-                ops.slice_copy(g.channels(ref.c0 - res.c0, ref.C), self.view(ref, grad=True), accumulate=acc)
+        res_view, res_acc = self._res_grad(b, g)
         pr, role = self._pair(idx)
         if pr is not None:
             # sibling pair (backward order: the follower B first, then the lead A): each module's BatchNorm backward writes its
@@ -1453,6 +1509,23 @@ class Engine:
             ref, acc = rec['x'], True
         ops.maxpool_bwd(self.view(rec['out'], grad=True), self.argmax[rec['idx']], self.view(ref, grad=True), rec['k'],
                         rec['stride'], rec['pad'], acc, self.pool_scratch)
+
+    def _b_dropout_bwd(self, b):
+        rec = b['fwd']
+        g = self.view(rec['out'], grad=True)
+        if rec['p'] == 0:
+            for ref, acc in b['dx']:
+                ops.slice_copy(g.channels(ref.c0 - rec['x'].c0, ref.C), self.view(ref, grad=True), accumulate=acc)
+            return
+        if len(b['dx']) == 1:
+            ref, acc = b['dx'][0]
+        else:
+            # (the mask goes by the index in the whole tensor: part of the input already holds a gradient -> zero the rest, then add)
+            for r, written in b['dx']:
+                if not written:
+                    ops.zero_view(self.view(r, grad=True), self.dummy)
+            ref, acc = rec['x'], True
+        ops.dropout_bwd(g, self.view(ref, grad=True), acc, rec['p'], self.rng, rec['idx'])
 
     def _b_upsample_bwd(self, b):
         rec = b['fwd']

@@ -8,7 +8,7 @@ the cfg is lowered to a list of operator records over pre-sized NHWC storages so
     concatenated storage (a tensor can live in one place only; a second cat copies);
   * [route] with groups / single-layer routes are views;
   * a [shortcut] whose left operand is a conv block consumed nowhere else is folded into that block's
-    BatchNorm+activation pass;
+    normalisation+activation pass, and so is a [dropout] behind a group-normalised conv block (and a [shortcut] behind that);
   * gradients of multi-consumer tensors are accumulated in place, the first writer storing and the
     later ones adding (tracked per storage channel at plan time).
 
@@ -34,8 +34,20 @@ def lower_blocks(blocks):
             k = int(blk['size'])
             m.update(n=conv_id, cin=ch, cout=int(blk['filters']), k=k, stride=int(blk['stride']),
                      pad=(k - 1) // 2 if int(blk['pad']) else 0, bn=int(blk['batch_normalize']),
-                     act=blk['activation'])
+                     act=blk['activation'], gn=int(blk.get('group_normalize', 0)))
+            # group_normalize=<groups>: statistics of one image and one group of channels in the place of batch_normalize
+            if m['gn'] and m['bn']:
+                raise ValueError('module %d: batch_normalize and group_normalize exclude each other' % i)
+            if m['gn'] < 0 or (m['gn'] and m['cout'] % m['gn']):
+                raise ValueError('module %d: %d filters do not divide into %d groups' % (i, m['cout'], m['gn']))
+            m['norm'] = bool(m['bn'] or m['gn'])
             ch = m['cout']
+        elif t == 'dropout':
+            m.update(p=float(blk.get('probability', 0.5)))
+            if not 0.0 <= m['p'] < 1.0:
+                raise ValueError('module %d: [dropout] probability %r' % (i, m['p']))
+            if i == 0 or mods[i - 1]['type'] == 'yolo' or (mods[i - 1]['type'] == 'convolutional' and not mods[i - 1]['norm']):
+                raise ValueError('module %d: a [dropout] block follows a normalised convolution or a structural block' % i)
         elif t == 'maxpool':
             m.update(k=int(blk['size']), stride=int(blk['stride']))
         elif t == 'upsample':
@@ -162,7 +174,7 @@ class Plan:
         consumers = {i: [] for i in range(n)}
         for i, m in enumerate(mods):
             t = m['type']
-            if t in ('convolutional', 'maxpool', 'upsample', 'yolo'):
+            if t in ('convolutional', 'maxpool', 'upsample', 'yolo', 'dropout'):
                 if i > 0:
                     consumers[self._resolve(i - 1)].append(i)
             elif t == 'route':
@@ -175,21 +187,30 @@ class Plan:
                 consumers[self._resolve(m['src'])].append(i)
         self.consumers = consumers
 
-        # shortcut fusion: left operand (module i-1) is a BN conv used by this shortcut only
+        # a dropout behind a group-normalised conv used by nothing else runs in that conv's normalisation pass
+        dropped_by = {}   # dropout idx -> conv idx
+        for i, m in enumerate(mods):
+            if m['type'] == 'dropout' and mods[i - 1]['type'] == 'convolutional' and mods[i - 1]['gn'] and consumers[i - 1] == [i]:
+                dropped_by[i] = i - 1
+        self.dropped_by = dropped_by
+
+        # shortcut fusion: left operand (module i-1) is a normalised conv used by this shortcut only, or such a conv's folded dropout
         fused_into = {}   # conv idx -> shortcut idx
         for i, m in enumerate(mods):
             if m['type'] == 'shortcut' and m['act'] == 'linear':
                 a = self._resolve(i - 1)
-                if a == i - 1 and mods[a]['type'] == 'convolutional' and mods[a]['bn'] and consumers[a] == [i] \
-                        and self._resolve(m['src']) != a:
-                    fused_into[a] = i
+                if a == i - 1 and consumers[a] == [i] and self._resolve(m['src']) != a:
+                    if mods[a]['type'] == 'convolutional' and mods[a]['norm']:
+                        fused_into[a] = i
+                    elif a in dropped_by:
+                        fused_into[dropped_by[a]] = i
         self.fused_into = fused_into
         fused_shortcuts = set(fused_into.values())
 
         # cat placement: a producer writes directly into the first concatenation that lists it
         placed = {}  # producer idx -> (cat idx, channel offset)
         cat_copy = {}  # cat idx -> [(src producer idx or ('view', ...), offset)]
-        producing = ('convolutional', 'maxpool', 'upsample', 'shortcut')
+        producing = ('convolutional', 'maxpool', 'upsample', 'shortcut', 'dropout')
         for i, m in enumerate(mods):
             if m['type'] != 'route' or (len(m['src']) == 1):
                 continue
@@ -197,7 +218,7 @@ class Plan:
             for s in m['src']:
                 b = self._resolve(s)
                 pm = mods[b]
-                ok = pm['type'] in producing and b not in placed and not (pm['type'] == 'convolutional' and not pm['bn'])
+                ok = pm['type'] in producing and b not in placed and not (pm['type'] == 'convolutional' and not pm['norm'])
                 if pm['type'] == 'convolutional' and b in fused_into:
                     ok = False  # its tensor does not exist on its own
                 if ok:
@@ -234,16 +255,22 @@ class Plan:
             if t == 'convolutional':
                 x = src_prev
                 rec = dict(op='conv', idx=i, n=m['n'], x=x, cin=m['cin'], cin_pad=x.C, cout=m['cout'], ks=m['k'],
-                           stride=m['stride'], pad=m['pad'], bn=bool(m['bn']), act=m['act'], H=H, W=W,
+                           stride=m['stride'], pad=m['pad'], bn=bool(m['bn']), gn=m['gn'], norm=m['norm'], act=m['act'], H=H, W=W,
                            xH=x.st.H, xW=x.st.W, first=(i == 0))
-                if m['bn']:
+                if m['norm']:
                     rec['raw'] = TRef(self._new_storage(H, W, C, 'raw'), 0, C)
+                    drop = i + 1 if dropped_by.get(i + 1) == i else None
+                    rec['drop'], rec['drop_id'] = (mods[drop]['p'], drop) if drop is not None else (0.0, 0)
                     if i in fused_into:
                         sc = fused_into[i]
                         out_ref = own_or_placed(sc)
                         rec['res'] = out[self._resolve(mods[sc]['src'])]
                         rec['out'] = out_ref
                         out[sc] = out_ref
+                        out[i] = None
+                    elif drop is not None:
+                        rec['res'] = None
+                        rec['out'] = out[drop] = own_or_placed(drop)
                         out[i] = None
                     else:
                         rec['res'] = None
@@ -259,6 +286,12 @@ class Plan:
                 k, s = m['k'], m['stride']
                 rec = dict(op='pool', idx=i, x=src_prev, out=own_or_placed(i), k=k, stride=s,
                            pad=pool_geometry(src_prev.st.H, k, s)[1])
+                out[i] = rec['out']
+                self.fwd.append(rec)
+            elif t == 'dropout':
+                if i in dropped_by:
+                    continue      # out[i] set by the conv (or, behind it, by the conv's shortcut)
+                rec = dict(op='dropout', idx=i, x=src_prev, out=own_or_placed(i), p=m['p'])
                 out[i] = rec['out']
                 self.fwd.append(rec)
             elif t == 'upsample':
@@ -298,6 +331,7 @@ class Plan:
                 out[i] = src_prev
         self.rows_total = rows
         self.out = out
+        self.has_dropout = any(m['type'] == 'dropout' and m['p'] > 0 for m in mods)
 
     # ---- backward ---------------------------------------------------------------------------------
     def _grad_runs(self, written, ref):
@@ -345,7 +379,7 @@ class Plan:
             if op == 'yolo':
                 continue
             if op == 'conv':
-                if not rec['bn']:
+                if not rec['norm']:
                     # head conv: gradient arrives as fp32 d(logits) from the loss kernel
                     b = dict(op='head_conv_bwd', fwd=rec)
                     b['dx'] = self._grad_runs(written, rec['x'])
@@ -361,7 +395,7 @@ class Plan:
                     b['res_runs'] = []
                 b['dx'] = [] if rec['first'] else self._grad_runs(written, rec['x'])
                 bwd.append(b)
-            elif op in ('pool', 'upsample', 'copy'):
+            elif op in ('pool', 'upsample', 'copy', 'dropout'):
                 if not self._has_grad(written, rec['out'], bwd):
                     continue
                 bwd.append(dict(op=op + '_bwd', fwd=rec, dx=self._grad_runs(written, rec['x'])))
@@ -384,7 +418,9 @@ class Plan:
         prev_conv = None     # bwd index of the latest conv_bwd / head_conv_bwd
         for bi, b in enumerate(self.bwd):
             op = b['op']
-            if op == 'conv_bwd':
+            if op == 'conv_bwd' and not b['fwd']['bn']:
+                b['sums_from'] = None      # (group norm: its sums are per image, its backward pass takes them itself)
+            elif op == 'conv_bwd':
                 L = b['fwd']
                 out = L['out']
                 writers = {last.get((out.st.sid, c)) for c in range(out.c0, out.c0 + out.C)}
@@ -409,7 +445,7 @@ class Plan:
             writes = []
             if op == 'conv_bwd':
                 writes += [(ref, 'res', ri) for ri, (ref, _) in enumerate(b['res_runs'])]
-            if op in ('conv_bwd', 'head_conv_bwd', 'pool_bwd', 'upsample_bwd', 'copy_bwd'):
+            if op in ('conv_bwd', 'head_conv_bwd', 'pool_bwd', 'upsample_bwd', 'copy_bwd', 'dropout_bwd'):
                 writes += [(ref, 'dgrad' if op.endswith('conv_bwd') else op, ri) for ri, (ref, _) in enumerate(b['dx'])]
             elif op == 'add_bwd':
                 writes += [(ref, op, ri) for ri, (ref, _) in enumerate(b['da'] + b['db'])]

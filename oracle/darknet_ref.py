@@ -15,7 +15,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import yolo_layer_ref
+from . import layers_ref, yolo_layer_ref
 
 
 def _layers(blocks):
@@ -33,8 +33,10 @@ def _layers(blocks):
             k = int(blk['size'])
             m.update(n=conv_id, cin=ch, cout=int(blk['filters']), k=k, stride=int(blk['stride']),
                      pad=(k - 1) // 2 if int(blk['pad']) else 0, bn=int(blk['batch_normalize']),
-                     act=blk['activation'])
+                     act=blk['activation'], gn=int(blk.get('group_normalize', 0)))
             ch = m['cout']
+        elif t == 'dropout':
+            m.update(p=float(blk.get('probability', 0.5)))
         elif t == 'maxpool':
             m.update(k=int(blk['size']), stride=int(blk['stride']))
         elif t == 'upsample':
@@ -79,17 +81,21 @@ class DarknetRef:
                 params['models.%d.bn%d.bias' % (i, n)] = (m['cout'],)
                 bufs['models.%d.bn%d.running_mean' % (i, n)] = (m['cout'],)
                 bufs['models.%d.bn%d.running_var' % (i, n)] = (m['cout'],)
+            elif m['gn']:
+                params['models.%d.gn%d.weight' % (i, n)] = (m['cout'],)
+                params['models.%d.gn%d.bias' % (i, n)] = (m['cout'],)
             else:
                 params['models.%d.conv%d.bias' % (i, n)] = (m['cout'],)
         return params, bufs
 
     def forward(self, params, x, targets=None, use_giou_loss=True, training=True, bufs=None,
-                keep=None, storage_round=None):
+                keep=None, storage_round=None, drop=None):
         """Returns (outputs[B,N,7+C], loss or None, [metrics per head]).  ``keep`` (a dict) receives
         intermediate activations by module index when given.  ``storage_round`` (a function tensor -> tensor, e.g. a
         float16 round trip) models 16-BIT STORAGE in this float32 arithmetic: it is applied to every convolution's input,
         weight and -- for BatchNorm layers -- output (the tensors a half-precision implementation keeps in memory; the
-        head logits stay float32).  The tests use it to tell what 16-bit rounding alone does to the reference's own
+        head logits stay float32).  ``drop`` = (seed, step) of the [dropout] masks in training (oracle/layers_ref.py; the layer id is
+        the module index).  The tests use it to tell what 16-bit rounding alone does to the reference's own
         function from what a kernel adds."""
         rnd = storage_round if storage_round is not None else (lambda t: t)
         img_size = x.shape[2]
@@ -105,7 +111,7 @@ class DarknetRef:
                 if storage_round is not None:      # 16-bit weight COPIES of float32 masters: the gradient stays float32
                     w = w + (rnd(w.detach()) - w.detach())
                 x = F.conv2d(rnd(x), w, b, m['stride'], m['pad'])
-                if m['bn'] and storage_round is not None:
+                if (m['bn'] or m['gn']) and storage_round is not None:
                     x = rnd(x)
                 if keep is not None:
                     keep[('raw', i)] = x
@@ -120,6 +126,8 @@ class DarknetRef:
                         x = F.batch_norm(x, rm, rv, g, be, True, 0.1, 1e-5)
                     else:
                         x = F.batch_norm(x, rm, rv, g, be, False, 0.1, 1e-5)
+                if m['gn']:
+                    x = F.group_norm(x, m['gn'], params['models.%d.gn%d.weight' % (i, n)], params['models.%d.gn%d.bias' % (i, n)], 1e-5)
                 if m['act'] == 'mish':
                     x = x * torch.tanh(F.softplus(x))
                 elif m['act'] == 'leaky':
@@ -138,6 +146,11 @@ class DarknetRef:
                         p1 = (k - 1) // 2
                         pads += [p1, p1 + 1 if ((n - 1) // s) != ((n + 2 * p - k) // s) else p1]
                     x = F.max_pool2d(F.pad(x, pads, mode='replicate'), k, stride=s)
+            elif t == 'dropout':
+                if training and m['p'] > 0:
+                    N, C, H, W = x.shape
+                    fac = layers_ref.drop_factor((N, H, W, C), int(m['p'] * 65536 + 0.5), drop[0], drop[1], i)
+                    x = x * fac.permute(0, 3, 1, 2).to(x.dtype)
             elif t == 'upsample':
                 x = x.repeat_interleave(m['stride'], 2).repeat_interleave(m['stride'], 3)
             elif t == 'route':
