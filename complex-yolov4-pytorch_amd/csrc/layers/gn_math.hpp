@@ -80,11 +80,11 @@ __device__ __forceinline__ float gn_act_grad(float z) {
 #pragma clang fp contract(off)
     if constexpr (ACT == CY_ACT_MISH) {
         const float n = gn_exp<FAST>(z);
-        const float w = n * (n + 2.f);
-        if constexpr (FAST) {
-            const float q = __builtin_amdgcn_rcpf(fmaf(w, 0.5f, 1.f));
-            return fmaf(z * (w - n), q * q, 1.f - q);
+        if constexpr (FAST) {      // z q^2 (w - n) = z (n q) (n q + q)
+            const float q = __builtin_amdgcn_rcpf(fmaf(n, fmaf(n, 0.5f, 1.f), 1.f)), t = n * q;
+            return fmaf(z * t, t + q, 1.f - q);
         }
+        const float w = n * (n + 2.f);
         const float t = w / (w + 2.f), q = 2.f / (w + 2.f);
         return fmaf(z * (w - n), q * q, t);      // (32 bits: tanh by itself, 1 - q cancels for large negative z)
     }

@@ -24,86 +24,115 @@ struct SumAcc {
     static __device__ __forceinline__ float2 out(const Sum& s) { return make_float2((float)s.u, (float)s.v); }
 };
 
-// R: 16-byte chunks of x and of dy a thread holds.  ONE: a chunk lies in one group.  x stays as stored; dz = drop(dy) act'(z) is formed once and kept in 32 bits -- the
-// activation's derivative is most of this kernel's arithmetic (an exponential and a reciprocal per element), and rounding dz to the
-// storage type would put its error into the sums.
+// R: 16-byte chunks of x and of dy a thread holds.  ONE: a chunk lies in one group.  x stays as stored; dz = drop(dy) act'(z) is formed
+// once and kept in 32 bits in dy's place -- the derivative is most of this kernel's arithmetic (an exponential and a reciprocal per
+// element), and rounding dz to the storage type would put its error into the sums.  Forming dz again after the meeting instead, with dy
+// as stored in the registers, leaves room for four waves a SIMD in place of three and is slower all the same, since blocks of one image
+// compute at the same time: 16 x 304 x 304 x 64 f16 216 us against 192, 16 x 76 x 76 x 256 bf16 with dropout 57 against 45.
 template <typename T, bool ONE, int ACT, bool DROP, int R>
 __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResShape sh, ResWork wk, DropRng rng) {
     constexpr int V = Elem<T>::CH;
     constexpr bool FAST = sizeof(T) == 2;
     __shared__ __attribute__((aligned(16))) float s_red[2 * GN_TB * V];
-    __shared__ float2 s_pair[ONE ? GN_TB : GN_TB * V], s_stat[ONE ? GN_TB : GN_TB * V];
+    extern __shared__ __attribute__((aligned(16))) float2 s_dyn[];
+    float2 *s_pair = s_dyn, *s_stat = s_dyn + sh.gps, *s_gb = s_stat + sh.gps;
     SumAcc::Sum* s_acc = reinterpret_cast<SumAcc::Sum*>(s_red);      // (after the block's own sums)
     static_assert(sizeof(SumAcc::Sum) * GN_TB <= sizeof(s_red), "accumulators fit where the sums were");
     const ResWhere w = res_where<R>(sh);
     const long img = (long)w.n * sh.HW, pmax = sh.HW - 1;
-    u32x4 d[R];
+    u32x4 d[R], g[R];
     float dz[R][V];
-    Norm<T, ACT> nm[V];
-    float sa[V], sb[V];
     int cnt = (w.px - w.row + sh.rows - 1) / sh.rows;
     cnt = !w.on || cnt < 0 ? 0 : cnt;
     DropKey key;
     if constexpr (DROP) key = drop_key(rng);
-    const int cc = w.chunk * V;
-    for (int g = threadIdx.x; g < sh.gps; g += GN_TB)
-        s_stat[g] = *reinterpret_cast<const float2*>(a.stats + 2 * ((long)w.n * sh.G + w.span * sh.gps + g));
+    const int nch = sh.width * V, c0 = w.span * nch, cc = w.chunk * V, lc0 = cc - c0;
+    {      // statistics, gamma and beta go to LDS.  They are asked for first: loads answer in order
+        const float2* st = reinterpret_cast<const float2*>(a.stats) + (long)w.n * sh.G + w.span * sh.gps;
+        const int t = threadIdx.x, ct = t < nch ? t : nch - 1, gt = t < sh.gps ? t : sh.gps - 1;
+        const float2 gb = make_float2(a.gamma[c0 + ct], a.beta[c0 + ct]), s0 = st[gt];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < V; ++i) sa[i] = sb[i] = 0.f;
-    if (w.on) {
-        u32x4 g[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {      // (beyond the image: its last pixel, left out below)
+        for (int r = 0; r < R; ++r) {      // (beyond the image: its last pixel, dy cleared below)
             long p = w.p0 + w.row + r * sh.rows;
             p = img + (p < pmax ? p : pmax);
             d[r] = *reinterpret_cast<const u32x4*>((const T*)a.x + p * a.ldx + cc);
             g[r] = *reinterpret_cast<const u32x4*>((const T*)a.dy + p * a.lddy + cc);
         }
+        // (nor is there a branch around the arithmetic: the loads would be moved into it, one behind the other: 200 us for the 192)
+        __builtin_amdgcn_sched_barrier(0);
+        s_gb[ct] = gb;
+        s_stat[gt] = s0;
+        for (int c = t + GN_TB; c < nch; c += GN_TB) s_gb[c] = make_float2(a.gamma[c0 + c], a.beta[c0 + c]);
+        for (int i = t + GN_TB; i < sh.gps; i += GN_TB) s_stat[i] = st[i];
+    }
+    __syncthreads();
+    if (a.resg) {      // the shortcut branch's gradient is dy itself
+        T* rg = (T*)a.resg + (img + w.p0 + w.row) * a.ldrg + cc;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float2 st = *reinterpret_cast<const float2*>(a.stats + 2 * ((long)w.n * sh.G + (cc + (ONE ? 0 : i)) / sh.Cg));
-            nm[i].set(st, a.gamma[cc + i], a.beta[cc + i]);
+        for (int r = 0; r < R; ++r)
+            if (r < cnt) {
+                u32x4 o = g[r];
+                if (a.res_accum) {
+                    float t[V], f[V];
+                    chunk_to_f32<T>(g[r], t);
+                    load_v<T, V>(rg + (long)r * sh.rows * a.ldrg, f);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) f[i] += t[i];
+                    o = f32_to_chunk<T>(f);
+                }
+                *reinterpret_cast<u32x4*>(rg + (long)r * sh.rows * a.ldrg) = o;
+            }
+    }
+    asm volatile("" : "+v"(cnt));      // (this and the ones below: what can be had again is not kept in registers)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (r >= cnt) g[r] = u32x4{0u, 0u, 0u, 0u};
+        if constexpr (DROP) g[r] = drop_raw<T>(key, rng.q, (unsigned long long)(img + w.p0 + w.row + r * sh.rows) * sh.C + cc, g[r]);
+        asm volatile("" : "+v"(g[r]));
+    }
+    // Four channels at a time: their constants are fetched from LDS, their four elements of a pixel hide each other's latency.
+    auto four = [](const u32x4& v, int h, float* f) {
+        float t[V];
+        chunk_to_f32<T>(FAST ? u32x4{v[h / 2], v[h / 2 + 1], 0u, 0u} : v, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = t[i];
+    };
+    auto grad = [&](float dy, float z) { return rounded((DROP ? dy * rng.scale : dy) * gn_act_grad<ACT, FAST>(z)); };
+#pragma unroll
+    for (int h = 0; h < V; h += 4) {
+        Norm<T, ACT> nm[4];
+        float sa[4], sb[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = lc0 + h + i;
+            nm[i].set(s_stat[(ONE ? lc0 : c) / sh.Cg], s_gb[c].x, s_gb[c].y);
+            sa[i] = sb[i] = 0.f;
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (r < cnt) {
-                const long p = img + w.p0 + w.row + r * sh.rows;
-                float f[V], t[V];
-                chunk_to_f32<T>(d[r], f);
-                chunk_to_f32<T>(g[r], t);
-                if (a.resg) {      // the shortcut branch's gradient is dy itself
-                    T* rg = (T*)a.resg + p * a.ldrg + cc;
-                    if (a.res_accum) {
-                        float o[V];
-                        load_v<T, V>(rg, o);
+            float f[4], t[4];
+            four(d[r], h, f);
+            four(g[r], h, t);
 #pragma unroll
-                        for (int i = 0; i < V; ++i) o[i] += t[i];
-                        store_v<T, V>(rg, o);
-                    } else {
-                        *reinterpret_cast<u32x4*>(rg) = g[r];
-                    }
-                }
-                if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)p * sh.C + cc, t);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float v = t[i] * gn_act_grad<ACT, FAST>(nm[i].z(f[i]));
-                    dz[r][i] = v;
-                    sa[i] += v;
-                    sb[i] += v * (f[i] - nm[i].mean);      // (times r when the rows are folded)
-                }
+            for (int i = 0; i < 4; ++i) {
+                const float v = grad(t[i], nm[i].z(f[i]));
+                dz[r][h + i] = v;
+                sa[i] += v;
+                sb[i] += v * (f[i] - nm[i].mean);      // (times r when the rows are folded)
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-    }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        s_red[(threadIdx.x * V + i) * 2] = sa[i];
-        s_red[(threadIdx.x * V + i) * 2 + 1] = sb[i];
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(s_red + (threadIdx.x * V + h + i) * 2) = make_float2(sa[i], sb[i]);
     }
+    asm volatile("" : "+v"(cnt));
+#pragma unroll
+    for (int r = 0; r < R; ++r) asm volatile("" : "+v"(d[r]));
     __syncthreads();
     // channels: a thread folds one channel's rows (neighbouring threads read neighbouring words), the sums go to the workspace for the
     // parameter gradients and, weighted with gamma, back into the first row
-    const int nch = sh.width * V;
-    float* chan = wk.chan + 2 * (((long)w.n * sh.nb + w.blk) * sh.C + (long)w.span * nch);
+    float* chan = wk.chan + 2 * (((long)w.n * sh.nb + w.blk) * sh.C + c0);
     for (int c = threadIdx.x; c < nch; c += GN_TB) {
         float u = 0.f, v = 0.f;
 #pragma unroll 8
@@ -114,7 +143,7 @@ __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResSha
         }
         v *= s_stat[c / sh.Cg].y;
         *reinterpret_cast<float2*>(chan + 2 * c) = make_float2(u, v);
-        const float gm = a.gamma[w.span * nch + c];
+        const float gm = s_gb[c].x;
         *reinterpret_cast<float2*>(s_red + 2 * c) = make_float2(u * gm, v * gm);
     }
     __syncthreads();
@@ -139,20 +168,31 @@ __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResSha
     bool ok = true;
     unsigned out = 0;
     if (sh.nb > 1) ok = cluster_meet<SumAcc>(sh, wk, w, SumAcc::Shape{}, s_pair, s_acc, &out, result, keep);
-    if (ok && cnt > 0) {
-        float2 k[V];
+    if (ok) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) k[i] = s_pair[(cc - w.span * nch + (ONE ? 0 : i)) / sh.Cg];
-        T* dx = (T*)a.dx + (img + w.p0 + w.row) * a.lddx + cc;
+        for (int h = 0; h < V; h += 4) {      // (dx takes x's place)
+            Norm<T, ACT> nm[4];
+            float2 k[4];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (r < cnt) {
-                float f[V];
-                chunk_to_f32<T>(d[r], f);
-#pragma unroll
-                for (int i = 0; i < V; ++i) f[i] = gn_dx(nm[i], k[i], f[i], dz[r][i]);
-                store_v<T, V>(dx + (long)r * sh.rows * a.lddx, f);
+            for (int i = 0; i < 4; ++i) {
+                const int c = lc0 + h + i, j = (ONE ? lc0 : c) / sh.Cg;
+                nm[i].set(s_stat[j], s_gb[c].x, s_gb[c].y);
+                k[i] = s_pair[j];
             }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float f[4], o[V] = {};
+                four(d[r], h, f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = gn_dx(nm[i], k[i], f[i], dz[r][h + i]);
+                const u32x4 b = f32_to_chunk<T>(o);
+                if constexpr (FAST) d[r][h / 2] = b[0], d[r][h / 2 + 1] = b[1];
+                else d[r] = b;
+                __builtin_amdgcn_sched_barrier(0);
+                if (h == V - 4 && r < cnt)
+                    *reinterpret_cast<u32x4*>((T*)a.dx + (img + w.p0 + w.row + (long)r * sh.rows) * a.lddx + cc) = d[r];
+            }
+        }
     }
     if (sh.nb == 1) return;
     cluster_leave<SumAcc>(sh, wk, w, SumAcc::Shape{}, s_acc, out, result, keep, [&](int blk, const unsigned long long* fin) {
@@ -170,7 +210,7 @@ __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResSha
                 const float2 st = s_stat[g];
                 Norm<T, ACT> one;
                 one.set(st, a.gamma[c + i], a.beta[c + i]);
-                f[i] = gn_dx(one, agent_load_pair(fin + g), f[i], t[i] * gn_act_grad<ACT, FAST>(one.z(f[i])));
+                f[i] = gn_dx(one, agent_load_pair(fin + g), f[i], rounded(t[i] * gn_act_grad<ACT, FAST>(one.z(f[i]))));
             }
             store_v<T, V>((T*)a.dx + pix * a.lddx + c, f);
         }
@@ -212,7 +252,8 @@ __global__ void __launch_bounds__(1024) gn_param_grad_kernel(const float* chan, 
 template <typename T, bool ONE, int ACT>
 int launch(const ResPlan& p, const ResBwd& a, const ResWork& wk, const DropRng& rng, hipStream_t s) {
     const dim3 grid((unsigned)((long)p.sh.N * p.sh.nspan * p.sh.nb));
-#define CY_R(D_, R_) hipLaunchKernelGGL((gn_bwd_resident_kernel<T, ONE, ACT, D_, R_>), grid, dim3(GN_TB), 0, s, a, p.sh, wk, rng)
+    const size_t lds = sizeof(float2) * (2 * p.sh.gps + p.sh.width * Elem<T>::CH);
+#define CY_R(D_, R_) hipLaunchKernelGGL((gn_bwd_resident_kernel<T, ONE, ACT, D_, R_>), grid, dim3(GN_TB), lds, s, a, p.sh, wk, rng)
     if (rng.q && p.R == 4) CY_R(true, 4);
     else if (rng.q) CY_R(true, 8);
     else if (p.R == 4) CY_R(false, 4);

@@ -57,7 +57,8 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     constexpr size_t SUMS = sizeof(float) * 2 * GN_TB * A, ACCS = sizeof(StatAcc::Sum) * GN_TB;
     __shared__ __attribute__((aligned(16))) char s_buf[SUMS > ACCS ? SUMS : ACCS];
     __shared__ float s_n[GN_TB];
-    __shared__ float2 s_pair[GN_TB * A], s_gb[GN_TB * V];
+    extern __shared__ __attribute__((aligned(16))) float2 s_dyn[];
+    float2 *s_pair = s_dyn, *s_gb = s_dyn + sh.gps;
     float *s_m = reinterpret_cast<float*>(s_buf), *s_q = s_m + GN_TB * A;
     StatAcc::Sum* s_acc = reinterpret_cast<StatAcc::Sum*>(s_buf);      // (after the block's own sums)
     const ResWhere w = res_where<R>(sh);
@@ -200,7 +201,8 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
 template <typename T, int A>
 int launch(const ResPlan& p, const ResFwd& a, const ResWork& wk, int act, const DropRng& rng, hipStream_t s) {
     const dim3 grid((unsigned)((long)p.sh.N * p.sh.nspan * p.sh.nb));
-#define CY_R(ACT_, D_, R_) hipLaunchKernelGGL((gn_fwd_resident_kernel<T, A, ACT_, D_, R_>), grid, dim3(GN_TB), 0, s, a, p.sh, wk, rng)
+    const size_t lds = sizeof(float2) * (p.sh.gps + p.sh.width * Elem<T>::CH);
+#define CY_R(ACT_, D_, R_) hipLaunchKernelGGL((gn_fwd_resident_kernel<T, A, ACT_, D_, R_>), grid, dim3(GN_TB), lds, s, a, p.sh, wk, rng)
 #define CY_ACT(ACT_)                               \
     if (rng.q && p.R == 8) CY_R(ACT_, true, 8);    \
     else if (rng.q) CY_R(ACT_, true, 16);          \

@@ -46,11 +46,13 @@ __device__ __forceinline__ Where where(const Shape& sh) {
     return w;
 }
 
-// A thread requests U pixels before it looks at the first.  Pixels behind the block's range are read as its last one and left out
-// afterwards: no branch between the loads.
-__device__ __forceinline__ long pixel(long p, int u, const Where& w) {
-    const long q = p + (long)u * w.rows;
-    return q < w.p1 ? q : w.p1 - 1;
+// Pixels of this thread in batches of U: batch(first pixel of the thread, distance) while U are left, then the rest one at a time.  Inside a batch
+// there is no branch, so that its loads stay in front of its arithmetic and are in flight together.
+template <int U, class Batch, class Single>
+__device__ __forceinline__ void each_pixel(const Where& w, Batch batch, Single single) {
+    long p = w.p0 + w.row;
+    for (; p + (long)(U - 1) * w.rows < w.p1; p += (long)U * w.rows) batch(p);
+    for (; p < w.p1; p += w.rows) single(p);
 }
 
 // Statistics of a column: NACC = 1 -- a chunk lies in one group, one (mean, sum of squares) per thread; NACC = V -- one per channel.
@@ -68,31 +70,37 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const T* x, int ldx, Shap
     int cnt = 0;
     if (w.on) {
         const T* src = x + (long)w.n * sh.HW * ldx + w.chunk * V;
-        for (long p = w.p0 + w.row; p < w.p1; p += (long)U * w.rows) {
-            Raw<T, V> in[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) in[u].load(src + pixel(p, u, w) * ldx);
+        auto take = [&](const Raw<T, V>& in) {
+            float f[V];
+            in.get(f);
             if (cnt == 0) {
-                float f[V];
-                in[0].get(f);
 #pragma unroll
                 for (int a = 0; a < NACC; ++a) K[a] = f[a];
             }
+            ++cnt;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (p + (long)u * w.rows >= w.p1) break;
-                float f[V];
-                in[u].get(f);
-                ++cnt;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const int a = NACC == 1 ? 0 : i;
-                    const float d = f[i] - K[a];
-                    s[a] += d;
-                    q[a] += d * d;
-                }
+            for (int i = 0; i < V; ++i) {
+                const int a = NACC == 1 ? 0 : i;
+                const float d = f[i] - K[a];
+                s[a] += d;
+                q[a] += d * d;
             }
-        }
+        };
+        each_pixel<U>(
+            w,
+            [&](long p) {
+                Raw<T, V> in[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) in[u].load(src + (p + u * w.rows) * ldx);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < U; ++u) take(in[u]);
+            },
+            [&](long p) {
+                Raw<T, V> in;
+                in.load(src + p * ldx);
+                take(in);
+            });
     }
     float n = (float)cnt * (V / NACC);
     float m[NACC];
@@ -184,32 +192,40 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const T* x, int ldx, T* y
         nm[i].set(*reinterpret_cast<const float2*>(stats + 2 * ((long)w.n * sh.G + c / sh.Cg)), gamma[c], beta[c]);
     }
     const long img = (long)w.n * sh.HW;
-    for (long p = w.p0 + w.row; p < w.p1; p += (long)U * w.rows) {
-        Raw<T, V> in[U], rin[U];
+    auto put = [&](long px, const Raw<T, V>& in, const Raw<T, V>& rin) {
+        float f[V];
+        in.get(f);
 #pragma unroll
-        for (int u = 0; u < U; ++u) in[u].load(x + (img + pixel(p, u, w)) * ldx + w.chunk * V);
+        for (int i = 0; i < V; ++i) f[i] = gn_act<ACT, FAST>(nm[i].z(f[i]));
+        if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, f);
         if (res) {
+            float r[V];
+            rin.get(r);
 #pragma unroll
-            for (int u = 0; u < U; ++u) rin[u].load(res + (img + pixel(p, u, w)) * ldres + w.chunk * V);
+            for (int i = 0; i < V; ++i) f[i] += r[i];
         }
+        store_v<T, V>(y + px * ldy + w.chunk * V, f);
+    };
+    each_pixel<U>(
+        w,
+        [&](long p) {
+            Raw<T, V> in[U], rin[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (p + (long)u * w.rows >= w.p1) break;
-            const long px = img + p + (long)u * w.rows;
-            float f[V];
-            in[u].get(f);
-#pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = gn_act<ACT, FAST>(nm[i].z(f[i]));
-            if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, f);
+            for (int u = 0; u < U; ++u) in[u].load(x + (img + p + u * w.rows) * ldx + w.chunk * V);
             if (res) {
-                float r[V];
-                rin[u].get(r);
 #pragma unroll
-                for (int i = 0; i < V; ++i) f[i] += r[i];
+                for (int u = 0; u < U; ++u) rin[u].load(res + (img + p + u * w.rows) * ldres + w.chunk * V);
             }
-            store_v<T, V>(y + px * ldy + w.chunk * V, f);
-        }
-    }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) put(img + p + u * w.rows, in[u], rin[u]);
+        },
+        [&](long p) {
+            Raw<T, V> in, rin;
+            in.load(x + (img + p) * ldx + w.chunk * V);
+            if (res) rin.load(res + (img + p) * ldres + w.chunk * V);
+            put(img + p, in, rin);
+        });
 }
 
 // Partial sums of dz and dz * xh per (image, pixel range, channel)
@@ -233,29 +249,37 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const T* x, int ldx, c
             nm[i].set(*reinterpret_cast<const float2*>(stats + 2 * ((long)w.n * sh.G + c / sh.Cg)), gamma[c], beta[c]);
         }
         const long img = (long)w.n * sh.HW;
-        for (long p = w.p0 + w.row; p < w.p1; p += (long)U * w.rows) {
-            Raw<T, V> in[U], gin[U];
+        auto take = [&](long px, const Raw<T, V>& in, const Raw<T, V>& gin) {
+            float f[V], g[V];
+            in.get(f);
+            gin.get(g);
+            if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, g);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                in[u].load(x + (img + pixel(p, u, w)) * ldx + w.chunk * V);
-                gin[u].load(dy + (img + pixel(p, u, w)) * lddy + w.chunk * V);
+            for (int i = 0; i < V; ++i) {
+                const float dz = rounded(g[i] * gn_act_grad<ACT, FAST>(nm[i].z(f[i])));
+                a[i] += dz;
+                b[i] += dz * (f[i] - nm[i].mean);
             }
+        };
+        each_pixel<U>(
+            w,
+            [&](long p) {
+                Raw<T, V> in[U], gin[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (p + (long)u * w.rows >= w.p1) break;
-                const long px = img + p + (long)u * w.rows;
-                float f[V], g[V];
-                in[u].get(f);
-                gin[u].get(g);
-                if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, g);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float dz = g[i] * gn_act_grad<ACT, FAST>(nm[i].z(f[i]));
-                    a[i] += dz;
-                    b[i] += dz * (f[i] - nm[i].mean);
+                for (int u = 0; u < U; ++u) {
+                    in[u].load(x + (img + p + u * w.rows) * ldx + w.chunk * V);
+                    gin[u].load(dy + (img + p + u * w.rows) * lddy + w.chunk * V);
                 }
-            }
-        }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < U; ++u) take(img + p + u * w.rows, in[u], gin[u]);
+            },
+            [&](long p) {
+                Raw<T, V> in, gin;
+                in.load(x + (img + p) * ldx + w.chunk * V);
+                gin.load(dy + (img + p) * lddy + w.chunk * V);
+                take(img + p, in, gin);
+            });
 #pragma unroll
         for (int i = 0; i < V; ++i) b[i] *= nm[i].r;
     }
@@ -354,38 +378,43 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const T* x, int ldx, 
         k[i] = gn_k01(nm[i].r, s12[j], s12[j + 1]);
     }
     const long img = (long)w.n * sh.HW;
-    for (long p = w.p0 + w.row; p < w.p1; p += (long)U * w.rows) {
-        Raw<T, V> in[U], gin[U];
+    auto put = [&](long px, const Raw<T, V>& in, const Raw<T, V>& gin) {
+        float f[V], g[V];
+        in.get(f);
+        gin.get(g);
+        if (resg) {      // the shortcut branch's gradient is dy itself
+            float o[V];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            in[u].load(x + (img + pixel(p, u, w)) * ldx + w.chunk * V);
-            gin[u].load(dy + (img + pixel(p, u, w)) * lddy + w.chunk * V);
+            for (int i = 0; i < V; ++i) o[i] = 0.f;
+            if (res_accum) load_v<T, V>(resg + px * ldrg + w.chunk * V, o);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] += g[i];
+            store_v<T, V>(resg + px * ldrg + w.chunk * V, o);
         }
+        if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, g);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (p + (long)u * w.rows >= w.p1) break;
-            const long px = img + p + (long)u * w.rows;
-            float f[V], g[V];
-            in[u].get(f);
-            gin[u].get(g);
-            if (resg) {      // the shortcut branch's gradient is dy itself
-                float o[V];
+        for (int i = 0; i < V; ++i) f[i] = gn_dx(nm[i], k[i], f[i], rounded(g[i] * gn_act_grad<ACT, FAST>(nm[i].z(f[i]))));
+        store_v<T, V>(dx + px * lddx + w.chunk * V, f);
+    };
+    each_pixel<U>(
+        w,
+        [&](long p) {
+            Raw<T, V> in[U], gin[U];
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = 0.f;
-                if (res_accum) load_v<T, V>(resg + px * ldrg + w.chunk * V, o);
-#pragma unroll
-                for (int i = 0; i < V; ++i) o[i] += g[i];
-                store_v<T, V>(resg + px * ldrg + w.chunk * V, o);
+            for (int u = 0; u < U; ++u) {
+                in[u].load(x + (img + p + u * w.rows) * ldx + w.chunk * V);
+                gin[u].load(dy + (img + p + u * w.rows) * lddy + w.chunk * V);
             }
-            if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)px * sh.C + w.chunk * V, g);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float dz = g[i] * gn_act_grad<ACT, FAST>(nm[i].z(f[i]));
-                f[i] = gn_dx(nm[i], k[i], f[i], dz);
-            }
-            store_v<T, V>(dx + px * lddx + w.chunk * V, f);
-        }
-    }
+            for (int u = 0; u < U; ++u) put(img + p + u * w.rows, in[u], gin[u]);
+        },
+        [&](long p) {
+            Raw<T, V> in, gin;
+            in.load(x + (img + p) * ldx + w.chunk * V);
+            gin.load(dy + (img + p) * lddy + w.chunk * V);
+            put(img + p, in, gin);
+        });
 }
 
 // no pixels at all: the parameter gradients are zero sums

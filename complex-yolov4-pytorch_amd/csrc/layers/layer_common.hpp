@@ -91,6 +91,23 @@ __device__ __forceinline__ void drop_apply(const DropKey& key, int q, float scal
     }
 }
 
+// The selection alone, on 16 bytes as they are stored: what is dropped becomes zero, what is kept is to be scaled.
+template <typename T>
+__device__ __forceinline__ u32x4 drop_raw(const DropKey& key, int q, unsigned long long e, u32x4 v) {
+    const u32x4 w = drop_words(key, e >> 3);
+    if constexpr (Elem<T>::CH == 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            v[k] &= (drop_half(w, 2 * k) >= q ? 0xFFFFu : 0u) | (drop_half(w, 2 * k + 1) >= q ? 0xFFFF0000u : 0u);
+    } else {
+        const bool up = (e >> 2) & 1;
+        const u32x4 h = {up ? w[2] : w[0], up ? w[3] : w[1], 0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = drop_half(h, i) >= q ? v[i] : 0u;
+    }
+    return v;
+}
+
 // host: drop probability in 65536ths -> generator arguments; false for arguments no kernel takes
 static inline bool make_drop(int q, const int64_t* state, int id, DropRng& r) {
     if (q < 0 || q > 65536 || (q > 0 && !state)) return false;
