@@ -47,6 +47,7 @@ struct ResWork {
     unsigned long long* pairs;       // [cluster][nb + nsub][group of the span]
     unsigned long long* fin;         // [cluster][group of the span]: results, for the block that finishes the list
     unsigned* list;                  // [cluster][block]
+    double* part;                    // backward: [channels / 8][slice][2][8], parameter gradients
     float* chan;                     // backward: [image][block][channel][2]
 };
 
@@ -310,5 +311,8 @@ struct ResBwd {
     float* ggamma; float* gbeta;
     float gscale; int accumulate;
 };
+// backward: the parameter gradients' rows (one per image and block) are added in this many slices, of at least 256 rows
+static inline int gn_param_slices(long rows) { return rows >= 16 * 256 ? 16 : rows < 512 ? 1 : (int)(rows / 256); }
+
 int gn_resident_fwd(const ResPlan& p, const ResFwd& a, const ResWork& wk, int act, int dtype, const DropRng& rng, hipStream_t s);
 int gn_resident_bwd(const ResPlan& p, const ResBwd& a, const ResWork& wk, int act, int dtype, const DropRng& rng, hipStream_t s);

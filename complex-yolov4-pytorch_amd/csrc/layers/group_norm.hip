@@ -343,6 +343,33 @@ __global__ void __launch_bounds__(256) gn_bwd_fold_kernel(const float* part, Sha
     }
 }
 
+// Parameter gradients from the images' channel sums, in double: a block takes eight channels, 32 lanes take images in turn and are added
+// in order.
+__device__ __forceinline__ void param_grads(int first, int N, int C, const float* chan, float* ggamma, float* gbeta, float gscale,
+                                            int accumulate) {
+    __shared__ double s_a[32][9], s_b[32][9];
+    const int k = threadIdx.x & 7, l = threadIdx.x >> 3, c = first + k;
+    double a = 0.0, b = 0.0;
+    if (c < C) {
+#pragma unroll 4
+        for (int n = l; n < N; n += 32) {
+            const float2 v = *reinterpret_cast<const float2*>(chan + 2 * ((long)n * C + c));
+            a += (double)v.x;
+            b += (double)v.y;
+        }
+    }
+    s_a[l][k] = a;
+    s_b[l][k] = b;
+    __syncthreads();
+    if (l > 0 || c >= C) return;
+    for (int i = 1; i < 32; ++i) {
+        a += s_a[i][k];
+        b += s_b[i][k];
+    }
+    if (gbeta) gbeta[c] = (accumulate ? gbeta[c] : 0.f) + gscale * (float)a;
+    if (ggamma) ggamma[c] = (accumulate ? ggamma[c] : 0.f) + gscale * (float)b;
+}
+
 template <typename T, int V, int ACT, bool DROP>
 __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const T* x, int ldx, const T* dy, int lddy, T* dx, int lddx, T* resg,
                                                           int ldrg, int res_accum, Shape sh, const float* stats,
@@ -351,21 +378,10 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(const T* x, int ldx, 
                                                           int accumulate, DropRng rng) {
     constexpr bool FAST = sizeof(T) == 2;
     constexpr int U = 4;
+    const long work = (long)sh.N * sh.nspan * sh.nblk;
+    if (blockIdx.x >= work) return param_grads((int)(blockIdx.x - work) * 8, sh.N, sh.C, chan, ggamma, gbeta, gscale, accumulate);
     const Where w = where(sh);
     if (!w.on) return;
-    if (w.n == 0 && w.blk == 0 && w.row == 0) {      // parameter gradients of this span: image order, double
-#pragma unroll 1
-        for (int i = 0; i < V; ++i) {
-            const int c = w.chunk * V + i;
-            double a = 0.0, b = 0.0;
-            for (int n = 0; n < sh.N; ++n) {
-                a += (double)chan[2 * ((long)n * sh.C + c)];
-                b += (double)chan[2 * ((long)n * sh.C + c) + 1];
-            }
-            if (gbeta) gbeta[c] = (accumulate ? gbeta[c] : 0.f) + gscale * (float)a;
-            if (ggamma) ggamma[c] = (accumulate ? ggamma[c] : 0.f) + gscale * (float)b;
-        }
-    }
     DropKey key;
     if constexpr (DROP) key = drop_key(rng);
     Norm<T, ACT> nm[V];
@@ -456,7 +472,9 @@ int64_t need_floats(const Shape& sh) {
 }
 
 constexpr int64_t MAX_BLOCKS = 1 << 24;      // a launch has fewer than 2^32 threads
-bool grid_ok(const Shape& sh) { return (int64_t)sh.N * sh.nspan * sh.nblk < MAX_BLOCKS && ((int64_t)sh.N * sh.G + 3) / 4 < MAX_BLOCKS; }
+bool grid_ok(const Shape& sh) {
+    return (int64_t)sh.N * sh.nspan * sh.nblk + sh.C / 8 + 1 < MAX_BLOCKS && ((int64_t)sh.N * sh.G + 3) / 4 < MAX_BLOCKS;
+}
 
 template <typename T, int V>
 int forward(const T* x, int ldx, T* y, int ldy, const T* res, int ldres, const Shape& sh, const float* gamma, const float* beta,
@@ -495,7 +513,8 @@ int backward(const T* x, int ldx, const T* dy, int lddy, T* dx, int lddx, T* res
     float* part = ws;
     float* s12 = part + 2 * (int64_t)sh.N * sh.nblk * sh.C;
     float* chan = s12 + 2 * (int64_t)sh.N * sh.G;
-    const dim3 grid((unsigned)((long)sh.N * sh.nspan * sh.nblk)), fgrid((unsigned)(((long)sh.N * sh.G + 3) / 4));
+    const dim3 grid((unsigned)((long)sh.N * sh.nspan * sh.nblk)), fgrid((unsigned)(((long)sh.N * sh.G + 3) / 4)),
+        agrid(grid.x + (ggamma || gbeta ? (sh.C + 7) / 8 : 0));
 #define CY_GNB(A_, D_)                                                                                                        \
     do {                                                                                                                      \
         hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, A_, D_>), grid, dim3(256), 0, s, x, ldx, dy, lddy, sh, stats, gamma, beta, \
@@ -503,7 +522,7 @@ int backward(const T* x, int ldx, const T* dy, int lddy, T* dx, int lddx, T* res
         CY_LAUNCH_CHECK();                                                                                                    \
         hipLaunchKernelGGL(gn_bwd_fold_kernel, fgrid, dim3(256), 0, s, part, sh, gamma, chan, s12);                            \
         CY_LAUNCH_CHECK();                                                                                                    \
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, A_, D_>), grid, dim3(256), 0, s, x, ldx, dy, lddy, dx, lddx, resg, ldrg, \
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, A_, D_>), agrid, dim3(256), 0, s, x, ldx, dy, lddy, dx, lddx, resg, ldrg, \
                            res_accum, sh, stats, gamma, beta, chan, s12, ggamma, gbeta, gscale, accumulate, rng);              \
     } while (0)
 #define CY_GNB_ACT(A_)             \
@@ -550,6 +569,31 @@ bool plan_width(int N, long HW, int C, int G, int V, int width, int R, int polls
     return true;
 }
 
+// Blocks that hold all pixels of their columns have nobody to meet: three to four microseconds less, where there are few enough of them
+// that a block's own time is what counts (f16, 8 chunks a thread unless said otherwise):
+//   1 x 19 x 19 x 1024 forward: 4 columns, alone 6.9 us; 8 columns, two blocks to an image 10.7     64 images: 27.6 against 22.4
+//   1 x 26 x 26 x 512: 2 columns 6.9; 8 columns 10.5      16 images: 4 columns, 16 chunks 11.1; 8 columns 13.4; 2 columns 15.1
+//   1 x 13 x 13 x 1024 backward: 4 columns, 4 chunks 9.4; 8 columns 12.5      16 images: 8 columns, 8 chunks 11.7; 8 columns, two blocks 15.1
+//   16 x 38 x 38 x 256 forward: 2 columns, 16 chunks (256 blocks) 16.1; 8 columns 13.4      4 images: 9.5 and 10.4
+// With a compute unit for each: as many blocks as there are compute units for, of four columns and more, or of two (up to 128 blocks).  With
+// more blocks than that: of four columns and more (backward, which reads twice as much: eight), the fewest first.
+bool plan_alone(int N, long HW, int C, int G, int V, bool bwd, int unit, int polls, ResPlan& p) {
+    const int cpr = C / V, most = bwd ? 8 : 16;
+    long best = 0;
+    for (int w = unit; w <= 8 && w <= cpr; w += unit) {
+        if (w < 2 || cpr % w) continue;
+        const long rows = GN_TB / w, blocks = (long)N * (cpr / w);
+        const int R = HW <= most / 2 * rows ? most / 2 : most;
+        if (HW > R * rows || (R == most && bwd && w < 4)) continue;
+        if (blocks > (w < 4 ? 128 : 256) && w < (bwd ? 8 : 4)) continue;
+        // (columns grow, blocks become fewer: the first of at most 256 wins, else the last)
+        if (best && best <= 256) continue;
+        if (!plan_width(N, HW, C, G, V, w, R, polls, p)) continue;
+        best = blocks;
+    }
+    return best > 0;
+}
+
 // Columns of a block: the number nearest to eight (one 128-byte line a pixel) that cuts the row into equal spans of whole groups: narrow
 // spans make small clusters, and a narrower one splits cache lines.  16 x 76 x 76 x 256 f16 forward: 4 columns 29.2 us, 8: 24.8, 16: 24.7,
 // 32: 25.6; backward 52.9, 44.2, 44.0, 49.0; 16 x 38 x 38 x 512 f16 backward with 64: 30.8, 8: 26.9.
@@ -560,6 +604,7 @@ bool plan_resident(int N, long HW, int C, int G, int V, bool bwd, ResPlan& p) {
     if (!cfg.mode || C % V) return false;
     const int Cg = C / G, unit = Cg / gcd(Cg, V);      // columns of the smallest span of whole groups and whole chunks
     const int cpr = C / V, units = cpr / unit, most = bwd ? 8 : 16;
+    if (!cfg.width && !cfg.R && plan_alone(N, HW, C, G, V, bwd, unit, cfg.polls, p)) return true;
     int tried = 0;      // (columns already looked at, as a lower bound of the distance from eight)
     for (;;) {
         int width = 0, best = 0;
@@ -584,10 +629,12 @@ bool plan_resident(int N, long HW, int C, int G, int V, bool bwd, ResPlan& p) {
     }
 }
 
+int64_t part_bytes(const ResPlan& p) { return (int64_t)gn_param_slices((long)p.sh.N * p.sh.nb) * ((p.sh.C + 7) / 8) * 16 * 8; }
+
 // bytes behind the part of a workspace that stays zero
 int64_t resident_bytes(const ResPlan& p) {
     const int64_t clusters = (int64_t)p.sh.N * p.sh.nspan;
-    return 8 * clusters * p.sh.gps + 8 * (int64_t)p.sh.N * p.sh.nb * p.sh.C + 4 * clusters * p.sh.nb;
+    return 8 * clusters * p.sh.gps + part_bytes(p) + 8 * (int64_t)p.sh.N * p.sh.nb * p.sh.C + 4 * clusters * p.sh.nb;
 }
 
 ResWork resident_work(const ResPlan& p, char* ws) {
@@ -596,7 +643,8 @@ ResWork resident_work(const ResPlan& p, char* ws) {
     w.counters = (unsigned*)ws;
     w.pairs = (unsigned long long*)(ws + GN_COUNTER_BYTES);
     w.fin = (unsigned long long*)(ws + GN_ZERO_BYTES);
-    w.chan = (float*)(w.fin + clusters * p.sh.gps);
+    w.part = (double*)(w.fin + clusters * p.sh.gps);
+    w.chan = (float*)((char*)w.part + part_bytes(p));
     w.list = (unsigned*)(w.chan + 2 * (int64_t)p.sh.N * p.sh.nb * p.sh.C);
     return w;
 }
