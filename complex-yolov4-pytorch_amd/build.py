@@ -12,8 +12,9 @@ SOURCES = ['conv_igemm.hip', 'conv_pipe.hip', 'conv_direct.hip', 'conv_wgrad.hip
 HEADERS = ['common.hpp', 'igemm_common.hpp', 'geometry.hpp', os.path.join(INCLUDE, 'cyolo_hip.h')]
 # Per-image layers (group norm, dropout): kernels nothing times or tunes, so they are not part of the sources the persisted conv choices
 # are stamped with (tune.py: csrc/*.h*) -- an edit here leaves that table valid.
-LAYER_SOURCES = ['layers/group_norm.hip', 'layers/gn_resident_fwd.hip', 'layers/gn_resident_bwd.hip', 'layers/dropout.hip']
-LAYER_HEADERS = ['layers/layer_common.hpp', 'layers/gn_math.hpp', 'layers/gn_resident.hpp']
+LAYER_SOURCES = (['layers/group_norm.hip', 'layers/dropout.hip'] +
+                 ['layers/gn_resident_%s_%s.hip' % (d, t) for d in ('fwd', 'bwd') for t in ('f16', 'bf16', 'f32')])
+LAYER_HEADERS = ['layers/' + h for h in ('layer_common.hpp', 'gn_math.hpp', 'gn_resident.hpp', 'gn_resident_fwd.hpp', 'gn_resident_bwd.hpp')]
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + INCLUDE, '-I' + CSRC, '-Wno-unused-value']
 # Per-file flags.  yolo_head.hip / riou_nms.hip: the per-target / per-pair kernels index small polygon arrays dynamically; with the
 # default promote-alloca budget they lived in scratch memory (368 / 880 bytes per lane) and assign / pairs were the only kernels of

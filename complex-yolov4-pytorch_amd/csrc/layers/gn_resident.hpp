@@ -32,10 +32,17 @@ constexpr int64_t GN_COUNTER_BYTES = (int64_t)GN_MAX_CLUSTERS * GN_WORDS * 4;
 constexpr int64_t GN_ZERO_BYTES = GN_COUNTER_BYTES + (int64_t)GN_MAX_PAIRS * 8;
 constexpr int GN_ONE_STEP = 4096;            // up to this many pairs (32 KB to read for every block) a cluster meets in one step
 
+// Chunks of V elements a thread holds at most: forward x, backward x and the 32-bit dz (half as many are built, too)
+template <int V>
+constexpr int GN_HELD_FWD = V == 1 ? 32 : 16;
+template <int V>
+constexpr int GN_HELD_BWD = V == 1 ? 32 : 8;
+static inline int gn_held(int V, bool bwd) { return V == 1 ? (bwd ? GN_HELD_BWD<1> : GN_HELD_FWD<1>) : bwd ? GN_HELD_BWD<8> : GN_HELD_FWD<8>; }
+
 struct ResShape {
     long HW;
     int N, C, G, Cg;
-    int width, nspan;      // chunk columns (16 bytes) of a span; spans per pixel row (width * nspan = C / V)
+    int width, nspan;      // chunk columns (V elements) of a span; spans per pixel row (width * nspan = C / V)
     int gps;               // groups of a span
     int rows, nb;          // pixels a block takes per step; blocks of a cluster
     int sub, nsub;         // two-step meeting: blocks that are combined first, how many such (0: one step)
@@ -292,7 +299,7 @@ __device__ __forceinline__ void cluster_leave(const ResShape& sh, const ResWork&
 // ---- host: launched from group_norm.hip ---------------------------------------------------------------------------------------
 struct ResPlan {
     ResShape sh;
-    int R;
+    int R, V;              // V: 16 bytes, or 1
 };
 struct ResFwd {
     const void* x; int ldx;
@@ -314,5 +321,11 @@ struct ResBwd {
 // backward: the parameter gradients' rows (one per image and block) are added in this many slices, of at least 256 rows
 static inline int gn_param_slices(long rows) { return rows >= 16 * 256 ? 16 : rows < 512 ? 1 : (int)(rows / 256); }
 
-int gn_resident_fwd(const ResPlan& p, const ResFwd& a, const ResWork& wk, int act, int dtype, const DropRng& rng, hipStream_t s);
-int gn_resident_bwd(const ResPlan& p, const ResBwd& a, const ResWork& wk, int act, int dtype, const DropRng& rng, hipStream_t s);
+#define CY_DECL(NAME_, ARGS_) int NAME_(const ResPlan& p, const ARGS_& a, const ResWork& wk, int act, const DropRng& rng, hipStream_t s)
+CY_DECL(gn_resident_fwd_f16, ResFwd);
+CY_DECL(gn_resident_fwd_bf16, ResFwd);
+CY_DECL(gn_resident_fwd_f32, ResFwd);
+CY_DECL(gn_resident_bwd_f16, ResBwd);
+CY_DECL(gn_resident_bwd_bf16, ResBwd);
+CY_DECL(gn_resident_bwd_f32, ResBwd);
+#undef CY_DECL

@@ -1,5 +1,6 @@
 // Backward group norm in one pass over x and dy (plus the fold of the parameter gradients).  See gn_resident.hpp for how the blocks of
-// an image meet.
+// an image meet.  (A source per element type includes this: they are built side by side.)
+#pragma once
 #include "gn_math.hpp"
 #include "gn_resident.hpp"
 
@@ -24,23 +25,23 @@ struct SumAcc {
     static __device__ __forceinline__ float2 out(const Sum& s) { return make_float2((float)s.u, (float)s.v); }
 };
 
-// R: 16-byte chunks of x and of dy a thread holds.  ONE: a chunk lies in one group.  x stays as stored; dz = drop(dy) act'(z) is formed
+// R: chunks of V elements of x and of dy a thread holds.  ONE: a chunk lies in one group.  x stays as stored; dz = drop(dy) act'(z) is formed
 // once and kept in 32 bits in dy's place -- the derivative is most of this kernel's arithmetic (an exponential and a reciprocal per
 // element), and rounding dz to the storage type would put its error into the sums.  Forming dz again after the meeting instead, with dy
 // as stored in the registers, leaves room for four waves a SIMD in place of three and is slower all the same, since blocks of one image
 // compute at the same time: 16 x 304 x 304 x 64 f16 216 us against 192, 16 x 76 x 76 x 256 bf16 with dropout 57 against 45.
-template <typename T, bool ONE, int ACT, bool DROP, int R>
+template <typename T, int V, bool ONE, int ACT, bool DROP, int R>
 __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResShape sh, ResWork wk, DropRng rng) {
-    constexpr int V = Elem<T>::CH;
+    constexpr int H = V < 4 ? V : 4;      // channels at a time
     constexpr bool FAST = sizeof(T) == 2;
-    __shared__ __attribute__((aligned(16))) float s_red[2 * GN_TB * V];
+    __shared__ __attribute__((aligned(16))) float s_red[V > 1 ? 2 * GN_TB * V : 4 * GN_TB];
     extern __shared__ __attribute__((aligned(16))) float2 s_dyn[];
     float2 *s_pair = s_dyn, *s_stat = s_dyn + sh.gps, *s_gb = s_stat + sh.gps;
     SumAcc::Sum* s_acc = reinterpret_cast<SumAcc::Sum*>(s_red);      // (after the block's own sums)
     static_assert(sizeof(SumAcc::Sum) * GN_TB <= sizeof(s_red), "accumulators fit where the sums were");
     const ResWhere w = res_where<R>(sh);
     const long img = (long)w.n * sh.HW, pmax = sh.HW - 1;
-    u32x4 d[R], g[R];
+    Raw<T, V> d[R], g[R];
     float dz[R][V];
     int cnt = (w.px - w.row + sh.rows - 1) / sh.rows;
     cnt = !w.on || cnt < 0 ? 0 : cnt;
@@ -56,8 +57,8 @@ __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResSha
         for (int r = 0; r < R; ++r) {      // (beyond the image: its last pixel, dy cleared below)
             long p = w.p0 + w.row + r * sh.rows;
             p = img + (p < pmax ? p : pmax);
-            d[r] = *reinterpret_cast<const u32x4*>((const T*)a.x + p * a.ldx + cc);
-            g[r] = *reinterpret_cast<const u32x4*>((const T*)a.dy + p * a.lddy + cc);
+            d[r].load((const T*)a.x + p * a.ldx + cc);
+            g[r].load((const T*)a.dy + p * a.lddy + cc);
         }
         // (nor is there a branch around the arithmetic: the loads would be moved into it, one behind the other: 200 us for the 192)
         __builtin_amdgcn_sched_barrier(0);
@@ -72,50 +73,45 @@ __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResSha
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (r < cnt) {
-                u32x4 o = g[r];
+                T* at = rg + (long)r * sh.rows * a.ldrg;
                 if (a.res_accum) {
                     float t[V], f[V];
-                    chunk_to_f32<T>(g[r], t);
-                    load_v<T, V>(rg + (long)r * sh.rows * a.ldrg, f);
+                    g[r].get(t);
+                    load_v<T, V>(at, f);
 #pragma unroll
                     for (int i = 0; i < V; ++i) f[i] += t[i];
-                    o = f32_to_chunk<T>(f);
+                    store_v<T, V>(at, f);
+                } else {
+                    g[r].store(at);
                 }
-                *reinterpret_cast<u32x4*>(rg + (long)r * sh.rows * a.ldrg) = o;
             }
     }
     asm volatile("" : "+v"(cnt));      // (this and the ones below: what can be had again is not kept in registers)
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (r >= cnt) g[r] = u32x4{0u, 0u, 0u, 0u};
-        if constexpr (DROP) g[r] = drop_raw<T>(key, rng.q, (unsigned long long)(img + w.p0 + w.row + r * sh.rows) * sh.C + cc, g[r]);
-        asm volatile("" : "+v"(g[r]));
+        if (r >= cnt) g[r].clear();
+        if constexpr (DROP) drop_raw(key, rng.q, (unsigned long long)(img + w.p0 + w.row + r * sh.rows) * sh.C + cc, g[r]);
+        g[r].pin();
     }
     // Four channels at a time: their constants are fetched from LDS, their four elements of a pixel hide each other's latency.
-    auto four = [](const u32x4& v, int h, float* f) {
-        float t[V];
-        chunk_to_f32<T>(FAST ? u32x4{v[h / 2], v[h / 2 + 1], 0u, 0u} : v, t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = t[i];
-    };
     auto grad = [&](float dy, float z) { return rounded((DROP ? dy * rng.scale : dy) * gn_act_grad<ACT, FAST>(z)); };
 #pragma unroll
-    for (int h = 0; h < V; h += 4) {
-        Norm<T, ACT> nm[4];
-        float sa[4], sb[4];
+    for (int h = 0; h < V; h += H) {
+        Norm<T, ACT> nm[H];
+        float sa[H], sb[H];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < H; ++i) {
             const int c = lc0 + h + i;
             nm[i].set(s_stat[(ONE ? lc0 : c) / sh.Cg], s_gb[c].x, s_gb[c].y);
             sa[i] = sb[i] = 0.f;
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            float f[4], t[4];
-            four(d[r], h, f);
-            four(g[r], h, t);
+            float f[H], t[H];
+            d[r].template part<H>(h, f);
+            g[r].template part<H>(h, t);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < H; ++i) {
                 const float v = grad(t[i], nm[i].z(f[i]));
                 dz[r][h + i] = v;
                 sa[i] += v;
@@ -124,11 +120,11 @@ __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResSha
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(s_red + (threadIdx.x * V + h + i) * 2) = make_float2(sa[i], sb[i]);
+        for (int i = 0; i < H; ++i) *reinterpret_cast<float2*>(s_red + (threadIdx.x * V + h + i) * 2) = make_float2(sa[i], sb[i]);
     }
     asm volatile("" : "+v"(cnt));
 #pragma unroll
-    for (int r = 0; r < R; ++r) asm volatile("" : "+v"(d[r]));
+    for (int r = 0; r < R; ++r) d[r].pin();
     __syncthreads();
     // channels: a thread folds one channel's rows (neighbouring threads read neighbouring words), the sums go to the workspace for the
     // parameter gradients and, weighted with gamma, back into the first row
@@ -170,27 +166,24 @@ __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResSha
     if (sh.nb > 1) ok = cluster_meet<SumAcc>(sh, wk, w, SumAcc::Shape{}, s_pair, s_acc, &out, result, keep);
     if (ok) {
 #pragma unroll
-        for (int h = 0; h < V; h += 4) {      // (dx takes x's place)
-            Norm<T, ACT> nm[4];
-            float2 k[4];
+        for (int h = 0; h < V; h += H) {      // (dx takes x's place)
+            Norm<T, ACT> nm[H];
+            float2 k[H];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < H; ++i) {
                 const int c = lc0 + h + i, j = (ONE ? lc0 : c) / sh.Cg;
                 nm[i].set(s_stat[j], s_gb[c].x, s_gb[c].y);
                 k[i] = s_pair[j];
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                float f[4], o[V] = {};
-                four(d[r], h, f);
+                float f[H];
+                d[r].template part<H>(h, f);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = gn_dx(nm[i], k[i], f[i], dz[r][h + i]);
-                const u32x4 b = f32_to_chunk<T>(o);
-                if constexpr (FAST) d[r][h / 2] = b[0], d[r][h / 2 + 1] = b[1];
-                else d[r] = b;
+                for (int i = 0; i < H; ++i) f[i] = gn_dx(nm[i], k[i], f[i], dz[r][h + i]);
+                d[r].template set_part<H>(h, f);
                 __builtin_amdgcn_sched_barrier(0);
-                if (h == V - 4 && r < cnt)
-                    *reinterpret_cast<u32x4*>((T*)a.dx + (img + w.p0 + w.row + (long)r * sh.rows) * a.lddx + cc) = d[r];
+                if (h == V - H && r < cnt) d[r].store((T*)a.dx + (img + w.p0 + w.row + (long)r * sh.rows) * a.lddx + cc);
             }
         }
     }
@@ -275,15 +268,16 @@ __global__ void __launch_bounds__(1024) gn_param_grad_kernel(const float* chan, 
     }
 }
 
-template <typename T, bool ONE, int ACT>
+template <typename T, int V, bool ONE, int ACT>
 int launch(const ResPlan& p, const ResBwd& a, const ResWork& wk, const DropRng& rng, hipStream_t s) {
+    constexpr int R = GN_HELD_BWD<V>;
     const dim3 grid((unsigned)((long)p.sh.N * p.sh.nspan * p.sh.nb));
-    const size_t lds = sizeof(float2) * (2 * p.sh.gps + p.sh.width * Elem<T>::CH);
-#define CY_R(D_, R_) hipLaunchKernelGGL((gn_bwd_resident_kernel<T, ONE, ACT, D_, R_>), grid, dim3(GN_TB), lds, s, a, p.sh, wk, rng)
-    if (rng.q && p.R == 4) CY_R(true, 4);
-    else if (rng.q) CY_R(true, 8);
-    else if (p.R == 4) CY_R(false, 4);
-    else CY_R(false, 8);
+    const size_t lds = sizeof(float2) * (2 * p.sh.gps + p.sh.width * V);
+#define CY_R(D_, R_) hipLaunchKernelGGL((gn_bwd_resident_kernel<T, V, ONE, ACT, D_, R_>), grid, dim3(GN_TB), lds, s, a, p.sh, wk, rng)
+    if (rng.q && p.R < R) CY_R(true, R / 2);
+    else if (rng.q) CY_R(true, R);
+    else if (p.R < R) CY_R(false, R / 2);
+    else CY_R(false, R);
 #undef CY_R
     CY_LAUNCH_CHECK();
     if (a.ggamma || a.gbeta) {
@@ -296,22 +290,19 @@ int launch(const ResPlan& p, const ResBwd& a, const ResWork& wk, const DropRng& 
     return 0;
 }
 
+template <typename T, int V, bool ONE>
+int launch_act(const ResPlan& p, const ResBwd& a, const ResWork& wk, int act, const DropRng& rng, hipStream_t s) {
+    if (act == CY_ACT_MISH) return launch<T, V, ONE, CY_ACT_MISH>(p, a, wk, rng, s);
+    if (act == CY_ACT_LEAKY) return launch<T, V, ONE, CY_ACT_LEAKY>(p, a, wk, rng, s);
+    return launch<T, V, ONE, CY_ACT_LINEAR>(p, a, wk, rng, s);
+}
+
 template <typename T>
 int launch_any(const ResPlan& p, const ResBwd& a, const ResWork& wk, int act, const DropRng& rng, hipStream_t s) {
-    if (p.sh.Cg % Elem<T>::CH == 0) {
-        if (act == CY_ACT_MISH) return launch<T, true, CY_ACT_MISH>(p, a, wk, rng, s);
-        if (act == CY_ACT_LEAKY) return launch<T, true, CY_ACT_LEAKY>(p, a, wk, rng, s);
-        return launch<T, true, CY_ACT_LINEAR>(p, a, wk, rng, s);
-    }
-    if (act == CY_ACT_MISH) return launch<T, false, CY_ACT_MISH>(p, a, wk, rng, s);
-    if (act == CY_ACT_LEAKY) return launch<T, false, CY_ACT_LEAKY>(p, a, wk, rng, s);
-    return launch<T, false, CY_ACT_LINEAR>(p, a, wk, rng, s);
+    constexpr int CH = Elem<T>::CH;
+    if (p.V == 1) return launch_act<T, 1, true>(p, a, wk, act, rng, s);
+    if (p.sh.Cg % CH == 0) return launch_act<T, CH, true>(p, a, wk, act, rng, s);
+    return launch_act<T, CH, false>(p, a, wk, act, rng, s);
 }
 
 }  // namespace
-
-int gn_resident_bwd(const ResPlan& p, const ResBwd& a, const ResWork& wk, int act, int dtype, const DropRng& rng, hipStream_t s) {
-    if (dtype == CY_F16) return launch_any<f16>(p, a, wk, act, rng, s);
-    if (dtype == CY_BF16) return launch_any<bf16>(p, a, wk, act, rng, s);
-    return launch_any<float>(p, a, wk, act, rng, s);
-}

@@ -1,13 +1,15 @@
-// Forward group norm in one launch: x is read once.  See gn_resident.hpp for how the blocks of an image meet.
+// Forward group norm in one launch: x is read once.  See gn_resident.hpp for how the blocks of an image meet.  (A source per
+// element type includes this: they are built side by side.)
+#pragma once
 #include "gn_math.hpp"
 #include "gn_resident.hpp"
 
 namespace {
 
-template <typename T, int ACT>
+template <typename T, int V, int ACT>
 __device__ __forceinline__ void finish(float* f, const Norm<T, ACT>* nm) {
 #pragma unroll
-    for (int i = 0; i < Elem<T>::CH; ++i) f[i] = gn_act<ACT, sizeof(T) == 2>(nm[i].z(f[i]));
+    for (int i = 0; i < V; ++i) f[i] = gn_act<ACT, sizeof(T) == 2>(nm[i].z(f[i]));
 }
 
 // (mean, centred sum of squares) of one group over entries of `per` blocks each, from block `first` on: a lane sums deviations of the
@@ -50,10 +52,10 @@ struct StatAcc {
     static __device__ __forceinline__ float2 out(const Sum& s) { return make_float2((float)s.mean, (float)s.m2); }
 };
 
-// R: 16-byte chunks of x a thread holds.  A: sums a thread keeps (gn_sums).
-template <typename T, int A, int ACT, bool DROP, int R>
+// R: chunks of V elements of x a thread holds.  A: sums a thread keeps (gn_sums).
+template <typename T, int V, int A, int ACT, bool DROP, int R>
 __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResShape sh, ResWork wk, DropRng rng) {
-    constexpr int V = Elem<T>::CH, PER = V / A;      // PER: channels of a chunk that share a sum
+    constexpr int PER = V / A;      // PER: channels of a chunk that share a sum
     constexpr size_t SUMS = sizeof(float) * 2 * GN_TB * A, ACCS = sizeof(StatAcc::Sum) * GN_TB;
     __shared__ __attribute__((aligned(16))) char s_buf[SUMS > ACCS ? SUMS : ACCS];
     __shared__ float s_n[GN_TB];
@@ -64,12 +66,12 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     const ResWhere w = res_where<R>(sh);
     const T* x = (const T*)a.x + (long)w.n * sh.HW * a.ldx;
     const long pmax = sh.HW - 1;
-    u32x4 d[R];
+    Raw<T, V> d[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {      // (pixels beyond the image are read as its last one and left out below: no branch between the loads)
         long p = w.p0 + w.row + r * sh.rows;
         p = p < pmax ? p : pmax;
-        d[r] = *reinterpret_cast<const u32x4*>(x + p * a.ldx + w.chunk * V);
+        d[r].load(x + p * a.ldx + w.chunk * V);
     }
     int cnt = (w.px - w.row + sh.rows - 1) / sh.rows;      // pixels of this thread
     cnt = !w.on || cnt < 0 ? 0 : cnt;
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     float K[A], s[A], q[A];
     {
         float f[V];
-        chunk_to_f32<T>(d[0], f);
+        d[0].get(f);
 #pragma unroll
         for (int j = 0; j < A; ++j) {
             K[j] = cnt > 0 ? f[j * PER] : 0.f;
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     for (int r = 0; r < R; ++r)
         if (r < cnt) {
             float f[V];
-            chunk_to_f32<T>(d[r], f);
+            d[r].get(f);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float t = f[i] - K[i / PER];
@@ -162,8 +164,8 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
         for (int r = 0; r < R; ++r)
             if (r < cnt) {
                 float f[V];
-                chunk_to_f32<T>(d[r], f);
-                finish<T, ACT>(f, nm);
+                d[r].get(f);
+                finish<T, V, ACT>(f, nm);
                 if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)(px0 + r * sh.rows) * sh.C + w.chunk * V, f);
                 if (a.res) {
                     float o[V];
@@ -172,6 +174,7 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
                     for (int i = 0; i < V; ++i) f[i] += o[i];
                 }
                 store_v<T, V>(y + (long)r * sh.rows * a.ldy, f);
+                if constexpr (V == 1 && DROP) __builtin_amdgcn_sched_barrier(0);      // (registers: not every element's generator at once)
             }
     }
     if (sh.nb == 1) return;
@@ -185,7 +188,7 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
             load_v<T, V>((const T*)a.x + pix * a.ldx + c, f);
 #pragma unroll
             for (int i = 0; i < V; ++i) nm[i].set(agent_load_pair(fin + (lc * V + i) / sh.Cg), a.gamma[c + i], a.beta[c + i]);
-            finish<T, ACT>(f, nm);
+            finish<T, V, ACT>(f, nm);
             if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)pix * sh.C + c, f);
             if (a.res) {
                 float o[V];
@@ -198,16 +201,17 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     });
 }
 
-template <typename T, int A>
+template <typename T, int V, int A>
 int launch(const ResPlan& p, const ResFwd& a, const ResWork& wk, int act, const DropRng& rng, hipStream_t s) {
+    constexpr int R = GN_HELD_FWD<V>;
     const dim3 grid((unsigned)((long)p.sh.N * p.sh.nspan * p.sh.nb));
-    const size_t lds = sizeof(float2) * (p.sh.gps + p.sh.width * Elem<T>::CH);
-#define CY_R(ACT_, D_, R_) hipLaunchKernelGGL((gn_fwd_resident_kernel<T, A, ACT_, D_, R_>), grid, dim3(GN_TB), lds, s, a, p.sh, wk, rng)
-#define CY_ACT(ACT_)                               \
-    if (rng.q && p.R == 8) CY_R(ACT_, true, 8);    \
-    else if (rng.q) CY_R(ACT_, true, 16);          \
-    else if (p.R == 8) CY_R(ACT_, false, 8);       \
-    else CY_R(ACT_, false, 16)
+    const size_t lds = sizeof(float2) * (p.sh.gps + p.sh.width * V);
+#define CY_R(ACT_, D_, R_) hipLaunchKernelGGL((gn_fwd_resident_kernel<T, V, A, ACT_, D_, R_>), grid, dim3(GN_TB), lds, s, a, p.sh, wk, rng)
+#define CY_ACT(ACT_)                                  \
+    if (rng.q && p.R < R) CY_R(ACT_, true, R / 2);    \
+    else if (rng.q) CY_R(ACT_, true, R);              \
+    else if (p.R < R) CY_R(ACT_, false, R / 2);       \
+    else CY_R(ACT_, false, R)
     if (act == CY_ACT_MISH) { CY_ACT(CY_ACT_MISH); }
     else if (act == CY_ACT_LEAKY) { CY_ACT(CY_ACT_LEAKY); }
     else { CY_ACT(CY_ACT_LINEAR); }
@@ -219,18 +223,14 @@ int launch(const ResPlan& p, const ResFwd& a, const ResWork& wk, int act, const 
 
 template <typename T>
 int launch_any(const ResPlan& p, const ResFwd& a, const ResWork& wk, int act, const DropRng& rng, hipStream_t s) {
-    const int A = gn_sums<Elem<T>::CH>(p.sh.Cg);
-    if (A == 1) return launch<T, 1>(p, a, wk, act, rng, s);
-    if (A == 2) return launch<T, 2>(p, a, wk, act, rng, s);
-    if constexpr (Elem<T>::CH == 8)
-        if (A == 8) return launch<T, 8>(p, a, wk, act, rng, s);
-    return launch<T, 4>(p, a, wk, act, rng, s);
+    constexpr int CH = Elem<T>::CH;
+    if (p.V == 1) return launch<T, 1, 1>(p, a, wk, act, rng, s);
+    const int A = gn_sums<CH>(p.sh.Cg);
+    if (A == 1) return launch<T, CH, 1>(p, a, wk, act, rng, s);
+    if (A == 2) return launch<T, CH, 2>(p, a, wk, act, rng, s);
+    if constexpr (CH == 8)
+        if (A == 8) return launch<T, CH, 8>(p, a, wk, act, rng, s);
+    return launch<T, CH, 4>(p, a, wk, act, rng, s);
 }
 
 }  // namespace
-
-int gn_resident_fwd(const ResPlan& p, const ResFwd& a, const ResWork& wk, int act, int dtype, const DropRng& rng, hipStream_t s) {
-    if (dtype == CY_F16) return launch_any<f16>(p, a, wk, act, rng, s);
-    if (dtype == CY_BF16) return launch_any<bf16>(p, a, wk, act, rng, s);
-    return launch_any<float>(p, a, wk, act, rng, s);
-}

@@ -1,0 +1,5 @@
+#include "gn_resident_fwd.hpp"
+
+int gn_resident_fwd_bf16(const ResPlan& p, const ResFwd& a, const ResWork& wk, int act, const DropRng& rng, hipStream_t s) {
+    return launch_any<bf16>(p, a, wk, act, rng, s);
+}

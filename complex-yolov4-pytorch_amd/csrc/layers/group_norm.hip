@@ -7,7 +7,7 @@
 //
 // This file: the choice of kernels, the C entry points, and the general kernels -- three launches per direction: partial sums per
 // (image, pixel range, column), a fold, the element pass -- for any row stride, alignment and channel count.  The one-launch kernels
-// are in gn_resident_*.  No floating-point atomics anywhere: a call's results do not depend on scheduling.
+// are in gn_resident*.  No floating-point atomics anywhere: a call's results do not depend on scheduling.
 //
 // A block works on one image n, one span of chunk columns and one range of pixels; thread = (row = t / width, chunk = t % width).
 #include "gn_math.hpp"
@@ -141,35 +141,46 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const T* x, int ldx, Shap
     }
 }
 
-// One wave per (image, group): the group's columns over all pixel ranges -> (mean, r).  Double, two passes over the partials
+// Sum over the block, the same in every thread
+__device__ __forceinline__ double block_sum_d(double v, double* s4) {
+    v = wave_sum_d(v);
+    if ((threadIdx.x & 63) == 0) s4[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    __syncthreads();
+    return v;
+}
+
+// One block per (image, group): the group's columns over all pixel ranges -> (mean, r).  Double, two passes over the partials
 // (weighted mean, then centred sum of squares).
 __global__ void __launch_bounds__(256) gn_fold_kernel(const float* part, Shape sh, int cols_per_group, int per_col, float eps,
                                                      float* stats) {
-    const long job = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (job >= (long)sh.N * sh.G) return;
+    __shared__ double s4[4];
+    const long job = blockIdx.x;
     const int n = (int)(job / sh.G), g = (int)(job % sh.G);
     const int cols = cols_per_group * sh.G;
     const float2* src = reinterpret_cast<const float2*>(part) + (long)n * sh.nblk * cols + g * cols_per_group;
     const int E = sh.nblk * cols_per_group;
     double sum = 0.0;
-    for (int i = lane; i < E; i += 64) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < E; i += 256) {
         const int blk = i / cols_per_group, k = i - blk * cols_per_group;
         const long px = blk == sh.nblk - 1 ? sh.HW - blk * sh.ppb : sh.ppb;
         sum += (double)px * (double)src[(long)blk * cols + k].x;
     }
     const double total = (double)sh.HW * cols_per_group;
-    const double mean = wave_sum_d(sum) / total;
+    const double mean = block_sum_d(sum, s4) / total;
     double m2 = 0.0;
-    for (int i = lane; i < E; i += 64) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < E; i += 256) {
         const int blk = i / cols_per_group, k = i - blk * cols_per_group;
         const long px = blk == sh.nblk - 1 ? sh.HW - blk * sh.ppb : sh.ppb;
         const float2 v = src[(long)blk * cols + k];
         const double d = (double)v.x - mean;
         m2 += (double)v.y + (double)px * per_col * d * d;
     }
-    m2 = wave_sum_d(m2);
-    if (lane == 0) {
+    m2 = block_sum_d(m2, s4);
+    if (threadIdx.x == 0) {
         stats[2 * job] = (float)mean;
         stats[2 * job + 1] = gn_rstd(m2 / (total * per_col), eps);
     }
@@ -303,40 +314,48 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const T* x, int ldx, c
     }
 }
 
-// One wave per (image, group): channel sums over the pixel ranges -> chan[n][c] = (sum dz, sum dz xh), and the group's S1, S2.
-// P = lanes side by side on channels (a power of two, at most 64); the other 64 / P take pixel ranges in turn.
+// One block per (image, group): channel sums over the pixel ranges -> chan[n][c] = (sum dz, sum dz xh), and the group's S1, S2.
+// P = threads side by side on channels (a power of two, at most 256); the other 256 / P take pixel ranges in turn.
 __global__ void __launch_bounds__(256) gn_bwd_fold_kernel(const float* part, Shape sh, const float* gamma, float* chan, float* s12) {
-    const long job = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (job >= (long)sh.N * sh.G) return;
-    const int n = (int)(job / sh.G), g = (int)(job % sh.G);
-    const int up = pow2_up(sh.Cg), P = up < 64 ? up : 64;
+    __shared__ double s_a[256], s_b[256], s4[4];
+    const long job = blockIdx.x;
+    const int t = threadIdx.x, n = (int)(job / sh.G), g = (int)(job % sh.G);
+    const int up = pow2_up(sh.Cg), P = up < 256 ? up : 256;
     const float2* src = reinterpret_cast<const float2*>(part) + (long)n * sh.nblk * sh.C + (long)g * sh.Cg;
     double s1 = 0.0, s2 = 0.0;
     for (int c0 = 0; c0 < sh.Cg; c0 += P) {
-        const int c = c0 + (lane & (P - 1));
+        const int c = c0 + (t & (P - 1));
         double a = 0.0, b = 0.0;
-        if (c < sh.Cg)
-            for (int k = lane / P; k < sh.nblk; k += 64 / P) {
+        if (c < sh.Cg) {
+#pragma unroll 4
+            for (int k = t / P; k < sh.nblk; k += 256 / P) {
                 const float2 v = src[(long)k * sh.C + c];
                 a += (double)v.x;
                 b += (double)v.y;
             }
-        for (int o = P; o < 64; o <<= 1) {
-            a += __shfl_xor(a, o, 64);
-            b += __shfl_xor(b, o, 64);
         }
-        if (c < sh.Cg && lane < P) {
+        s_a[t] = a;
+        s_b[t] = b;
+        __syncthreads();
+        for (int h = 128; h >= P; h >>= 1) {
+            if (t < h) {
+                s_a[t] += s_a[t + h];
+                s_b[t] += s_b[t + h];
+            }
+            __syncthreads();
+        }
+        if (c < sh.Cg && t < P) {
             const int cc = g * sh.Cg + c;
-            chan[2 * ((long)n * sh.C + cc)] = (float)a;
-            chan[2 * ((long)n * sh.C + cc) + 1] = (float)b;
-            s1 += (double)gamma[cc] * a;
-            s2 += (double)gamma[cc] * b;
+            chan[2 * ((long)n * sh.C + cc)] = (float)s_a[t];
+            chan[2 * ((long)n * sh.C + cc) + 1] = (float)s_b[t];
+            s1 += (double)gamma[cc] * s_a[t];
+            s2 += (double)gamma[cc] * s_b[t];
         }
+        __syncthreads();
     }
-    s1 = wave_sum_d(s1);
-    s2 = wave_sum_d(s2);
-    if (lane == 0) {
+    s1 = block_sum_d(s1, s4);
+    s2 = block_sum_d(s2, s4);
+    if (t == 0) {
         const double m = (double)sh.HW * sh.Cg;
         s12[2 * job] = (float)(s1 / m);
         s12[2 * job + 1] = (float)(s2 / m);
@@ -473,7 +492,7 @@ int64_t need_floats(const Shape& sh) {
 
 constexpr int64_t MAX_BLOCKS = 1 << 24;      // a launch has fewer than 2^32 threads
 bool grid_ok(const Shape& sh) {
-    return (int64_t)sh.N * sh.nspan * sh.nblk + sh.C / 8 + 1 < MAX_BLOCKS && ((int64_t)sh.N * sh.G + 3) / 4 < MAX_BLOCKS;
+    return (int64_t)sh.N * sh.nspan * sh.nblk + sh.C / 8 + 1 < MAX_BLOCKS && (int64_t)sh.N * sh.G < MAX_BLOCKS;
 }
 
 template <typename T, int V>
@@ -482,7 +501,7 @@ int forward(const T* x, int ldx, T* y, int ldy, const T* res, int ldres, const S
     if (!grid_ok(sh)) return CY_ERR_ARG;
     float* part = ws;
     if (!stats) stats = ws + 2 * (int64_t)sh.N * sh.nblk * sh.C;
-    const dim3 grid((unsigned)((long)sh.N * sh.nspan * sh.nblk)), fgrid((unsigned)(((long)sh.N * sh.G + 3) / 4));
+    const dim3 grid((unsigned)((long)sh.N * sh.nspan * sh.nblk)), fgrid((unsigned)((long)sh.N * sh.G));
     const bool one = sh.Cg % V == 0;
     if (one) hipLaunchKernelGGL((gn_stats_kernel<T, V, 1>), grid, dim3(256), 0, s, x, ldx, sh, part);
     else hipLaunchKernelGGL((gn_stats_kernel<T, V, V>), grid, dim3(256), 0, s, x, ldx, sh, part);
@@ -513,7 +532,7 @@ int backward(const T* x, int ldx, const T* dy, int lddy, T* dx, int lddx, T* res
     float* part = ws;
     float* s12 = part + 2 * (int64_t)sh.N * sh.nblk * sh.C;
     float* chan = s12 + 2 * (int64_t)sh.N * sh.G;
-    const dim3 grid((unsigned)((long)sh.N * sh.nspan * sh.nblk)), fgrid((unsigned)(((long)sh.N * sh.G + 3) / 4)),
+    const dim3 grid((unsigned)((long)sh.N * sh.nspan * sh.nblk)), fgrid((unsigned)((long)sh.N * sh.G)),
         agrid(grid.x + (ggamma || gbeta ? (sh.C + 7) / 8 : 0));
 #define CY_GNB(A_, D_)                                                                                                        \
     do {                                                                                                                      \
@@ -549,10 +568,14 @@ Config g_cfg = {1, POLLS, 0, 0};
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
-// One shape of blocks: `width` 16-byte columns, R chunks to a thread.  false: its blocks cannot meet.
+// Columns of V elements that make about a 128-byte line
+int columns(int V) { return V == 1 ? 64 : 8; }
+
+// One shape of blocks: `width` columns, R chunks to a thread.  false: its blocks cannot meet.
 bool plan_width(int N, long HW, int C, int G, int V, int width, int R, int polls, ResPlan& p) {
     const int Cg = C / G, gps = width * V / Cg;
     p.R = R;
+    p.V = V;
     p.sh = ResShape{HW, N, C, G, Cg, width, C / V / width, gps, GN_TB / width, 0, 0, 0, polls};
     const long nb = (HW + (long)R * p.sh.rows - 1) / ((long)R * p.sh.rows), clusters = (long)N * p.sh.nspan;
     if (nb > 512 || clusters * nb >= MAX_BLOCKS) return false;      // (half of the blocks that fit on the chip)
@@ -578,14 +601,14 @@ bool plan_width(int N, long HW, int C, int G, int V, int width, int R, int polls
 // With a compute unit for each: as many blocks as there are compute units for, of four columns and more, or of two (up to 128 blocks).  With
 // more blocks than that: of four columns and more (backward, which reads twice as much: eight), the fewest first.
 bool plan_alone(int N, long HW, int C, int G, int V, bool bwd, int unit, int polls, ResPlan& p) {
-    const int cpr = C / V, most = bwd ? 8 : 16;
+    const int cpr = C / V, most = gn_held(V, bwd), line = columns(V);
     long best = 0;
-    for (int w = unit; w <= 8 && w <= cpr; w += unit) {
-        if (w < 2 || cpr % w) continue;
+    for (int w = unit; w <= line && w <= cpr; w += unit) {
+        if (w < (V == 1 ? 4 : 2) || cpr % w) continue;
         const long rows = GN_TB / w, blocks = (long)N * (cpr / w);
         const int R = HW <= most / 2 * rows ? most / 2 : most;
-        if (HW > R * rows || (R == most && bwd && w < 4)) continue;
-        if (blocks > (w < 4 ? 128 : 256) && w < (bwd ? 8 : 4)) continue;
+        if (HW > R * rows || (R == most && bwd && w < line / 2)) continue;
+        if (blocks > (w < line / 2 ? 128 : 256) && w < (bwd ? line : line / 2)) continue;
         // (columns grow, blocks become fewer: the first of at most 256 wins, else the last)
         if (best && best <= 256) continue;
         if (!plan_width(N, HW, C, G, V, w, R, polls, p)) continue;
@@ -599,21 +622,25 @@ bool plan_alone(int N, long HW, int C, int G, int V, bool bwd, int unit, int pol
 // 32: 25.6; backward 52.9, 44.2, 44.0, 49.0; 16 x 38 x 38 x 512 f16 backward with 64: 30.8, 8: 26.9.
 // Chunks of a thread: 16 (backward 8: x and the 32-bit dz), half of that where fewer than 512 blocks would be left for 256 compute units:
 // 16 x 38 x 38 x 512 f16 forward (384 blocks at 16) 19.0 us with 16, 16.5 with 8; 16 x 76 x 76 x 256 f16 (768) 24.8 with 16, 28.8 with 8.
+// Element by element (rows that do not start on 16 bytes): the same in 64 columns and twice, backward four times, as many elements as there
+// would be chunks.  Up to 2048 blocks -- as many as fit at a time, about: 16 x 38 x 38 x 255 f32 forward (720 blocks) 21.6 us, three
+// launches 30.8; 16 x 76 x 76 x 255 f16 (2900 blocks) 55 and 38.
 bool plan_resident(int N, long HW, int C, int G, int V, bool bwd, ResPlan& p) {
     const Config cfg = g_cfg;
     if (!cfg.mode || C % V) return false;
     const int Cg = C / G, unit = Cg / gcd(Cg, V);      // columns of the smallest span of whole groups and whole chunks
-    const int cpr = C / V, units = cpr / unit, most = bwd ? 8 : 16;
+    const int cpr = C / V, units = cpr / unit, most = gn_held(V, bwd), line = columns(V);
     if (!cfg.width && !cfg.R && plan_alone(N, HW, C, G, V, bwd, unit, cfg.polls, p)) return true;
     int tried = 0;      // (columns already looked at, as a lower bound of the distance from eight)
     for (;;) {
         int width = 0, best = 0;
         for (int i = 1; i <= units && i * unit <= GN_TB; ++i) {
             if (units % i) continue;
-            const int w = i * unit, far = w >= 8 ? w * 8 : 8 * 8 * 8 / w;      // 64 times the factor between w and 8
-            if (far * 2 + (w < 8) > tried && (!width || far * 2 + (w < 8) < best)) {
+            const int w = i * unit, far = w >= line ? 64 * w / line : 64 * line / w;      // 64 times the factor between the two
+            const int key = far * 2 + (w < line);
+            if (key > tried && (!width || key < best)) {
                 width = w;
-                best = far * 2 + (w < 8);
+                best = key;
             }
         }
         if (!width) return false;
@@ -624,7 +651,7 @@ bool plan_resident(int N, long HW, int C, int G, int V, bool bwd, ResPlan& p) {
             const long ppb = (long)most * (GN_TB / width);
             if ((long)N * (cpr / width) * ((HW + ppb - 1) / ppb) < 512) R = most / 2;
         }
-        if (plan_width(N, HW, C, G, V, width, R, cfg.polls, p)) return true;
+        if (plan_width(N, HW, C, G, V, width, R, cfg.polls, p)) return V > 1 || cfg.width || (long)N * p.sh.nspan * p.sh.nb <= 2048;
         if (cfg.width) return false;
     }
 }
@@ -663,9 +690,10 @@ int forward_any(const void* x, int ldx, void* y, int ldy, const void* res, int l
     if (!aligned_to(x, sizeof(T)) || !aligned_to(y, sizeof(T)) || !aligned_to(res, sizeof(T))) return CY_ERR_ARG;
     const bool vec = C % CH == 0 && rows16<T>(x, ldx) && rows16<T>(y, ldy) && rows16<T>(res, ldres);
     ResPlan rp;
-    if (vec && plan_resident(N, HW, C, G, CH, false, rp)) {
+    if (plan_resident(N, HW, C, G, vec ? CH : 1, false, rp)) {
         if (ws_bytes < GN_ZERO_BYTES + resident_bytes(rp)) return CY_ERR_ARG;
-        return gn_resident_fwd(rp, ResFwd{x, ldx, y, ldy, res, ldres, gamma, beta, eps, stats}, resident_work(rp, ws), act, Elem<T>::DT, rng, s);
+        const auto call = sizeof(T) == 4 ? gn_resident_fwd_f32 : Elem<T>::DT == CY_F16 ? gn_resident_fwd_f16 : gn_resident_fwd_bf16;
+        return call(rp, ResFwd{x, ldx, y, ldy, res, ldres, gamma, beta, eps, stats}, resident_work(rp, ws), act, rng, s);
     }
     const Shape sh = make_shape(N, HW, C, G, vec ? CH : 1);
     if (ws_bytes < GN_ZERO_BYTES + 4 * need_floats(sh)) return CY_ERR_ARG;
@@ -683,10 +711,11 @@ int backward_any(const void* x, int ldx, const void* dy, int lddy, void* dx, int
         return CY_ERR_ARG;
     const bool vec = C % CH == 0 && rows16<T>(x, ldx) && rows16<T>(dy, lddy) && rows16<T>(dx, lddx) && rows16<T>(resg, ldrg);
     ResPlan rp;
-    if (vec && plan_resident(N, HW, C, G, CH, true, rp)) {
+    if (plan_resident(N, HW, C, G, vec ? CH : 1, true, rp)) {
         if (ws_bytes < GN_ZERO_BYTES + resident_bytes(rp)) return CY_ERR_ARG;
-        return gn_resident_bwd(rp, ResBwd{x, ldx, dy, lddy, dx, lddx, resg, ldrg, res_accum, gamma, beta, stats, ggamma, gbeta, gscale, accumulate},
-                               resident_work(rp, ws), act, Elem<T>::DT, rng, s);
+        const auto call = sizeof(T) == 4 ? gn_resident_bwd_f32 : Elem<T>::DT == CY_F16 ? gn_resident_bwd_f16 : gn_resident_bwd_bf16;
+        return call(rp, ResBwd{x, ldx, dy, lddy, dx, lddx, resg, ldrg, res_accum, gamma, beta, stats, ggamma, gbeta, gscale, accumulate},
+                    resident_work(rp, ws), act, rng, s);
     }
     const Shape sh = make_shape(N, HW, C, G, vec ? CH : 1);
     if (ws_bytes < GN_ZERO_BYTES + 4 * need_floats(sh)) return CY_ERR_ARG;
@@ -703,14 +732,15 @@ int backward_any(const void* x, int ldx, const void* dy, int lddy, void* dx, int
 extern "C" int64_t cy_gn_workspace(int N, int64_t HW, int C, int groups, int dtype) {
     if (!sizes_ok(N, HW, C, groups, dtype)) return CY_ERR_ARG;
     if (N == 0 || HW == 0) return GN_ZERO_BYTES;
-    int64_t most = 4 * need_floats(make_shape(N, (long)HW, C, groups, 1));      // (whichever kernels a call's pointers allow)
     const int ch = dtype == CY_F32 ? 4 : 8;
-    if (C % ch == 0) {
-        const int64_t v = 4 * need_floats(make_shape(N, (long)HW, C, groups, ch));
+    int64_t most = 0;      // (whichever kernels a call's pointers allow)
+    for (int V : {1, ch}) {
+        if (C % V) continue;
+        const int64_t v = 4 * need_floats(make_shape(N, (long)HW, C, groups, V));
         if (v > most) most = v;
         for (int bwd = 0; bwd < 2; ++bwd) {
             ResPlan p;
-            if (plan_resident(N, (long)HW, C, groups, ch, bwd != 0, p) && resident_bytes(p) > most) most = resident_bytes(p);
+            if (plan_resident(N, (long)HW, C, groups, V, bwd != 0, p) && resident_bytes(p) > most) most = resident_bytes(p);
         }
     }
     return GN_ZERO_BYTES + most;

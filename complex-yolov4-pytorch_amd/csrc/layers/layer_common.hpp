@@ -14,18 +14,53 @@ __device__ __forceinline__ void store_v(T* p, const float* f) {
     else *reinterpret_cast<u32x4*>(p) = f32_to_chunk<T>(f);
 }
 
-// the same in two steps, so that several loads can be in flight before the first is looked at
+// The same in two steps, so that several loads can be in flight before the first is looked at.  part / set_part: H (4, or all) elements
+// from h on.  pin: what was computed from the value is not kept in registers beyond this point, it is computed again.
 template <typename T, int V>
 struct Raw {
     u32x4 v;
     __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const u32x4*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<u32x4*>(p) = v; }
     __device__ __forceinline__ void get(float* f) const { chunk_to_f32<T>(v, f); }
+    __device__ __forceinline__ void clear() { v = u32x4{0u, 0u, 0u, 0u}; }
+    __device__ __forceinline__ void pin() { asm volatile("" : "+v"(v)); }
+    template <int H>
+    __device__ __forceinline__ void part(int h, float* f) const {
+        float t[V];
+        chunk_to_f32<T>(V == 8 ? u32x4{v[h / 2], v[h / 2 + 1], 0u, 0u} : v, t);
+#pragma unroll
+        for (int i = 0; i < H; ++i) f[i] = t[i];
+    }
+    template <int H>
+    __device__ __forceinline__ void set_part(int h, const float* f) {
+        float t[V] = {};
+#pragma unroll
+        for (int i = 0; i < H; ++i) t[i] = f[i];
+        const u32x4 b = f32_to_chunk<T>(t);
+        if constexpr (V == 8) v[h / 2] = b[0], v[h / 2 + 1] = b[1];
+        else v = b;
+    }
 };
 template <typename T>
 struct Raw<T, 1> {
     T v;
     __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ void store(T* p) const { *p = v; }
     __device__ __forceinline__ void get(float* f) const { f[0] = (float)v; }
+    __device__ __forceinline__ void clear() { v = (T)0.f; }
+    __device__ __forceinline__ void pin() {
+        if constexpr (sizeof(T) == 4) {
+            asm volatile("" : "+v"(v));
+        } else {
+            unsigned u = __builtin_bit_cast(unsigned short, v);
+            asm volatile("" : "+v"(u));
+            v = __builtin_bit_cast(T, (unsigned short)u);
+        }
+    }
+    template <int H>
+    __device__ __forceinline__ void part(int, float* f) const { f[0] = (float)v; }
+    template <int H>
+    __device__ __forceinline__ void set_part(int, const float* f) { v = (T)f[0]; }
 };
 
 // ---- dropout generator ---------------------------------------------------------------------------------------------------
@@ -70,6 +105,13 @@ __device__ __forceinline__ u32x4 drop_words(const DropKey& key, unsigned long lo
 
 __device__ __forceinline__ int drop_half(const u32x4& w, int j) { return (int)((w[j >> 1] >> (16 * (j & 1))) & 0xFFFFu); }
 
+// the same for a j that is not a constant
+__device__ __forceinline__ int drop_one(const u32x4& w, int j) {
+    const unsigned lo = (j & 2) ? w[1] : w[0], hi = (j & 2) ? w[3] : w[2];
+    const unsigned x = (j & 4) ? hi : lo;
+    return (int)((j & 1) ? x >> 16 : x & 0xFFFFu);
+}
+
 // f[i] = kept ? f[i] * scale : 0 for the V elements from dense element index e on.  A selection, not a product: what is in a dropped
 // place (a NaN too) does not come through.  e is a multiple of V.
 template <int V>
@@ -84,28 +126,26 @@ __device__ __forceinline__ void drop_apply(const DropKey& key, int q, float scal
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = drop_half(h, i) >= q ? f[i] * scale : 0.f;
     } else {
-        const int j = (int)(e & 7);
-        const unsigned lo = (j & 2) ? w[1] : w[0], hi = (j & 2) ? w[3] : w[2];
-        const unsigned x = (j & 4) ? hi : lo;
-        f[0] = (int)((j & 1) ? x >> 16 : x & 0xFFFFu) >= q ? f[0] * scale : 0.f;
+        f[0] = drop_one(w, (int)(e & 7)) >= q ? f[0] * scale : 0.f;
     }
 }
 
-// The selection alone, on 16 bytes as they are stored: what is dropped becomes zero, what is kept is to be scaled.
-template <typename T>
-__device__ __forceinline__ u32x4 drop_raw(const DropKey& key, int q, unsigned long long e, u32x4 v) {
+// The selection alone, on a chunk as it is stored: what is dropped becomes zero, what is kept is to be scaled.
+template <typename T, int V>
+__device__ __forceinline__ void drop_raw(const DropKey& key, int q, unsigned long long e, Raw<T, V>& x) {
     const u32x4 w = drop_words(key, e >> 3);
-    if constexpr (Elem<T>::CH == 8) {
+    if constexpr (V == 8) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            v[k] &= (drop_half(w, 2 * k) >= q ? 0xFFFFu : 0u) | (drop_half(w, 2 * k + 1) >= q ? 0xFFFF0000u : 0u);
-    } else {
+            x.v[k] &= (drop_half(w, 2 * k) >= q ? 0xFFFFu : 0u) | (drop_half(w, 2 * k + 1) >= q ? 0xFFFF0000u : 0u);
+    } else if constexpr (V == 4) {
         const bool up = (e >> 2) & 1;
         const u32x4 h = {up ? w[2] : w[0], up ? w[3] : w[1], 0u, 0u};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = drop_half(h, i) >= q ? v[i] : 0u;
+        for (int i = 0; i < 4; ++i) x.v[i] = drop_half(h, i) >= q ? x.v[i] : 0u;
+    } else {
+        if (drop_one(w, (int)(e & 7)) < q) x.clear();
     }
-    return v;
 }
 
 // host: drop probability in 65536ths -> generator arguments; false for arguments no kernel takes
