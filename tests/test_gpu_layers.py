@@ -227,6 +227,50 @@ def test_statistics_beside_a_large_mean(shape, dt, kernels):
     _close(st[..., 1], n['rstd'], n['rstd'] * (512 * E + merged), 'r')
 
 
+@pytest.mark.parametrize('config', [{}, dict(mode=0), dict(width=256)], ids=['policy', 'general', 'wide'])
+@pytest.mark.parametrize('shape,dt', [
+    ((300, 11, 100, 4, 1, 0, 0), CY_F32),       # 600 blocks' sums per channel: parameter gradients in two slices
+    ((16, 512, 512, 4, 2, 0, 0), CY_F32),       # 2048: in eight
+    ((70, 9, 9, 24, 8, 0, 0), CY_BF16),         # more images than lanes that add them
+    ((16, 76, 76, 255, 17, 0, 0), CY_F16),      # element by element, more blocks than fit at a time
+    ((2, 7, 9, 2048, 2048, 0, 0), CY_F16),      # the widest block: 2048 groups of one channel
+    ((9, 19, 19, 512, 32, 0, 0), CY_BF16),      # blocks alone with their columns, more of them than compute units
+], ids=lambda v: '%dx%dx%dx%d_g%d' % v[:5] if isinstance(v, tuple) else NAMES[v])
+def test_many_images_blocks_and_columns(shape, dt, config):
+    """Against the 64-bit formulas on the device.  A sum's depth here: at most 64 values of a thread and 256 rows of a block (the rest is
+    in double), so 320 e of the sum of magnitudes; a column of the general kernels adds up to 512 pixels per thread and eight levels."""
+    N, H, W, C, G, pad, off = shape
+    x, dy, _, gamma, beta = (t.to(DEV) for t in _problem(shape, dt, 31))
+    xs, dys = View(x, 0, N, H, W, C, C, dt), View(dy, 0, N, H, W, C, C, dt)
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    stats, gg = torch.empty(N, G, 2, device=DEV), torch.empty(2, C, device=DEV)
+    ops.gn_config(**config)
+    try:
+        ws = _workspace(N, H, W, C, G, dt)
+        ops.gn_act_fwd(xs, View(y, 0, N, H, W, C, C, dt), None, gamma, beta, G, EPS, 2, stats, ws)
+        ops.gn_act_bwd(xs, dys, View(dx, 0, N, H, W, C, C, dt), None, False, gamma, beta, stats, G, 2, gg[0], gg[1], 1.0, False, ws)
+        torch.cuda.synchronize()
+        assert int(ws[:COUNTERS].max()) == 0
+    finally:
+        ops.gn_config()
+    one = torch.ones((), dtype=torch.float64, device=DEV)
+    want, n = ref.gn_act(x, gamma, beta, G, EPS, 2, one)
+    per_c = lambda t: t.repeat_interleave(C // G, -1)[:, None, :]      # noqa: E731
+    xe = 64 * E * (per_c(n['rstd'] * (1 + n['mean'].abs())) * (1 + x.double().abs()))      # error of xh
+    _close(y, want, _stored(want, dt) + 1.1 * (xe * gamma.double().abs() + 16 * E * (beta.double().abs() + n['z'].abs())) + 8 * E * want.abs(), 'y')
+    o = ref.gn_act_grad(x, dy, gamma, beta, G, EPS, 2, one)
+    ze = xe * gamma.double().abs() + 16 * E * (beta.double().abs() + n['z'].abs())
+    dze = 3 * ze * dy.double().abs() + 16 * E * o['dz'].abs()
+    depth = (520 if config.get('mode') == 0 else 320) * E
+    for k, name, t, err in ((0, 'ggamma', o['dz'] * o['xh'], dze * o['xh'].abs() + (o['dz'].abs() + dze) * xe), (1, 'gbeta', o['dz'], dze)):
+        _close(gg[k], t.sum((0, 1)), err.sum((0, 1)) + depth * t.abs().sum((0, 1)), name)
+    grp = lambda t: t.reshape(N, H * W, G, -1).mean((1, 3))      # noqa: E731
+    he, h = dze * gamma.double().abs(), o['h'].abs()
+    sums = per_c(grp(he) + depth * grp(h)) + o['xh'].abs() * per_c(grp(he * o['xh'].abs() + (h + he) * xe) + depth * grp(h * o['xh'].abs()))
+    tol = per_c(n['rstd']) * (he + sums + xe * per_c(o['s2'].abs()) + 16 * E * (h + per_c(grp(h)))) + 80 * E * o['dx'].abs()
+    _close(dx, o['dx'], tol + _stored(o['dx'], dt), 'dx')
+
+
 def test_non_finite_values_stay_in_their_group():
     N, H, W, C, G = 2, 6, 6, 32, 4
     x, dy, _, gamma, beta = _problem((N, H, W, C, G, 0, 0), CY_F16, 3)
