@@ -559,47 +559,59 @@ def bn_act_bwd_apply(x, dy, dx, res_grad, res_accum, mean, invstd, scale, shift,
 # ---- per-image layers: group norm + activation, dropout ---------------------------------------------
 
 # (A layer call on a small map is shorter on the GPU than in this file: pointers travel as plain integers, each argument is looked at
-# once, and the stream is asked for through torch's raw-handle query.  15 -> 7 us of host time a call.)
+# once, and the stream is asked for through torch's raw-handle query.  15 -> 7 to 8 us of host time a call, the launch among them.)
 
-def _layer_device(who, first):
-    """The index of the device the call runs on: that of its first view, which has to be the current one (the launch goes to its
-    current stream)."""
+def _layer_first(who, v):
+    """The first view of a call -> (index of the device, pixels, type of the storage, address).  The call runs on its device, which has to
+    be the current one (the launch goes to its current stream)."""
     _require_gpu()
-    buf = first.buf
+    buf = v.buf
     dev = buf.get_device()
     if dev != torch.cuda.current_device():
         check_device_tensor(buf, who)
         raise CyoloError('%s: the tensors are on %s, the current device is cuda:%d' % (who, buf.device, torch.cuda.current_device()))
-    if buf.dtype is not _TORCH_DT.get(first.dt):
-        raise CyoloError('%s: %s of type %r' % (who, _view_str(first), first.dt))
-    return dev
+    kind = buf.dtype
+    if kind is not _TORCH_DT.get(v.dt):
+        raise CyoloError('%s: %s of type %r' % (who, _view_str(v), v.dt))
+    m, ld, off = v.N * v.H * v.W, v.ld, v.off
+    if ld < v.C or off < 0 or (m and off + (m - 1) * ld + v.C > buf.numel()) or not buf.is_contiguous():
+        raise _beyond(who, v)
+    return dev, m, kind, buf.data_ptr() + off * _ELSIZE[v.dt]
 
 
-def _layer_view(who, v, first, dev):
-    """Address of a view of ``first``'s shape, type and device that lies inside its buffer (None: None)."""
+def _layer_view(who, v, first, dev, m, kind):
+    """Address of a view of ``first``'s shape, type and device (what _layer_first gave) that lies inside its buffer (None: None)."""
     if v is None:
         return None
-    buf = v.buf
-    if (v.C != first.C or v.W != first.W or v.H != first.H or v.N != first.N or v.dt != first.dt or buf.dtype is not first.buf.dtype
+    buf, C, ld, off = v.buf, v.C, v.ld, v.off
+    if (C != first.C or v.W != first.W or v.H != first.H or v.N != first.N or v.dt != first.dt or buf.dtype is not kind
             or buf.get_device() != dev):
         raise CyoloError('%s: views differ in shape, type or device: %s and %s' % (who, _view_str(first), _view_str(v)))
-    m = v.N * v.H * v.W
-    if v.ld < v.C or v.off < 0 or (m and v.off + (m - 1) * v.ld + v.C > buf.numel()) or not buf.is_contiguous():
-        raise CyoloError('%s: %s reaches beyond its buffer of %d elements' % (who, _view_str(v), buf.numel()))
-    return buf.data_ptr() + v.off * _ELSIZE[v.dt]
+    if ld < C or off < 0 or (m and off + (m - 1) * ld + C > buf.numel()) or not buf.is_contiguous():
+        raise _beyond(who, v)
+    return buf.data_ptr() + off * _ELSIZE[v.dt] if off else buf.data_ptr()
+
+
+def _beyond(who, v):
+    return CyoloError('%s: %s reaches beyond its buffer of %d elements' % (who, _view_str(v), v.buf.numel()))
+
+
+_F32 = torch.float32
 
 
 def _layer_floats(who, name, t, n, dev):
     """Address of n contiguous float32 values (None: None)."""
     if t is None:
         return None
-    if t.dtype is not torch.float32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+    if t.dtype is not _F32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
         raise CyoloError('%s: %s must be %d contiguous float32 values on the views\' device' % (who, name, n))
     return t.data_ptr()
 
 
 def _layer_drop(who, p, rng, dev):
     """-> (65536ths, address of the generator state)."""
+    if rng is None and p == 0:
+        return 0, None
     q = dropout_q(p)
     if rng is None:
         if q:
@@ -665,32 +677,34 @@ def _check_gn(who, x, gamma, beta, groups, act, ws, dev):
 def gn_act_fwd(x, y, res, gamma, beta, groups, eps, act, stats, ws, drop=0.0, rng=None, drop_id=0):
     """y = res + dropout(act(group norm of x)); stats: float32 [N, groups, 2] (mean, 1 / deviation) for gn_act_bwd, or None."""
     who = 'gn_act_fwd'
-    dev = _layer_device(who, x)
+    dev, m, kind, px = _layer_first(who, x)
     _check_gn(who, x, gamma, beta, groups, act, ws, dev)
     if y is None or not eps >= 0.0:
         raise CyoloError('gn_act_fwd: an output and eps >= 0 are needed')
     q, state = _layer_drop(who, drop, rng, dev)
-    lib().call('cy_gn_act_fwd', _layer_view(who, x, x, dev), x.ld, _layer_view(who, y, x, dev), y.ld, _layer_view(who, res, x, dev),
-               res.ld if res is not None else 0, x.N, x.H * x.W, x.C, groups, _layer_floats(who, 'gamma', gamma, x.C, dev),
-               _layer_floats(who, 'beta', beta, x.C, dev), eps, act, x.dt, _layer_floats(who, 'stats', stats, 2 * x.N * groups, dev), q,
-               state, drop_id, ws.data_ptr(), ws.numel() * ws.element_size(), _layer_stream(dev))
+    N, C = x.N, x.C
+    lib().call('cy_gn_act_fwd', px, x.ld, _layer_view(who, y, x, dev, m, kind), y.ld, _layer_view(who, res, x, dev, m, kind),
+               res.ld if res is not None else 0, N, x.H * x.W, C, groups, _layer_floats(who, 'gamma', gamma, C, dev),
+               _layer_floats(who, 'beta', beta, C, dev), eps, act, x.dt, _layer_floats(who, 'stats', stats, 2 * N * groups, dev), q,
+               state, drop_id, ws.data_ptr(), ws.nbytes, _layer_stream(dev))
 
 
 def gn_act_bwd(x, dy, dx, res_grad, res_accum, gamma, beta, stats, groups, act, ggamma, gbeta, gscale, accumulate, ws, drop=0.0, rng=None,
                drop_id=0):
     """dx (may be dy), ggamma / gbeta (+)= gscale * sums (None: not wanted); res_grad (+)= dy, the shortcut branch's gradient."""
     who = 'gn_act_bwd'
-    dev = _layer_device(who, x)
+    dev, m, kind, px = _layer_first(who, x)
     _check_gn(who, x, gamma, beta, groups, act, ws, dev)
     if dy is None or dx is None or stats is None:
         raise CyoloError('gn_act_bwd: dy, dx and the statistics of the forward pass are needed')
     q, state = _layer_drop(who, drop, rng, dev)
-    lib().call('cy_gn_act_bwd', _layer_view(who, x, x, dev), x.ld, _layer_view(who, dy, x, dev), dy.ld, _layer_view(who, dx, x, dev), dx.ld,
-               _layer_view(who, res_grad, x, dev), res_grad.ld if res_grad is not None else 0, 1 if res_accum else 0, x.N, x.H * x.W, x.C,
-               groups, _layer_floats(who, 'gamma', gamma, x.C, dev), _layer_floats(who, 'beta', beta, x.C, dev),
-               _layer_floats(who, 'stats', stats, 2 * x.N * groups, dev), act, x.dt, _layer_floats(who, 'ggamma', ggamma, x.C, dev),
-               _layer_floats(who, 'gbeta', gbeta, x.C, dev), gscale, 1 if accumulate else 0, q, state, drop_id, ws.data_ptr(),
-               ws.numel() * ws.element_size(), _layer_stream(dev))
+    N, C = x.N, x.C
+    lib().call('cy_gn_act_bwd', px, x.ld, _layer_view(who, dy, x, dev, m, kind), dy.ld, _layer_view(who, dx, x, dev, m, kind), dx.ld,
+               _layer_view(who, res_grad, x, dev, m, kind), res_grad.ld if res_grad is not None else 0, 1 if res_accum else 0, N,
+               x.H * x.W, C, groups, _layer_floats(who, 'gamma', gamma, C, dev), _layer_floats(who, 'beta', beta, C, dev),
+               _layer_floats(who, 'stats', stats, 2 * N * groups, dev), act, x.dt, _layer_floats(who, 'ggamma', ggamma, C, dev),
+               _layer_floats(who, 'gbeta', gbeta, C, dev), gscale, 1 if accumulate else 0, q, state, drop_id, ws.data_ptr(), ws.nbytes,
+               _layer_stream(dev))
 
 
 def dropout_fwd(x, y, p, rng, drop_id=0):
@@ -704,12 +718,12 @@ def dropout_bwd(dy, dx, accumulate, p, rng, drop_id=0):
 
 
 def _dropout(who, x, y, p, rng, drop_id, accumulate):
-    dev = _layer_device(who, x)
+    dev, m, kind, px = _layer_first(who, x)
     if rng is None or y is None:
         raise CyoloError('%s: an output and the generator state (ops.dropout_state) are needed' % who)
     q, state = _layer_drop(who, p, rng, dev)
-    lib().call('cy_dropout', _layer_view(who, x, x, dev), x.ld, _layer_view(who, y, x, dev), y.ld, x.N * x.H * x.W, x.C, q, state, drop_id,
-               accumulate, x.dt, _layer_stream(dev))
+    lib().call('cy_dropout', px, x.ld, _layer_view(who, y, x, dev, m, kind), y.ld, m, x.C, q, state, drop_id, accumulate, x.dt,
+               _layer_stream(dev))
 
 
 def maxpool_argmax_bytes(N, H, OH, OW, C):
