@@ -6,13 +6,6 @@
 #pragma once
 #include "layer_common.hpp"
 
-// The value as it stands: keeps the conversion to 16 bits that follows from being merged into the multiply-add before it (one rounding
-// instead of two, where the compiler finds it: two kernels' stored values would differ in their last bit).
-__device__ __forceinline__ float rounded(float v) {
-    asm("" : "+v"(v));
-    return v;
-}
-
 // ---- normalisation -----------------------------------------------------------------------------------------------------------
 // Per channel, from the group's (mean, r) and (gamma, beta): z(x) and the deviation from the mean.
 //

@@ -75,6 +75,18 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     }
     int cnt = (w.px - w.row + sh.rows - 1) / sh.rows;      // pixels of this thread
     cnt = !w.on || cnt < 0 ? 0 : cnt;
+    // the generator runs while the loads are under way
+    DropKey key;
+    DropBits<R * V> keep_mask;
+    if constexpr (DROP) {
+        key = drop_key(rng);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            keep_mask.template put<V>(key, rng.q, ((unsigned long long)((long)w.n * sh.HW + w.p0 + w.row) + r * sh.rows) * sh.C + w.chunk * V, r * V);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
     // gamma and beta wait in LDS (in registers they would cost a wave of occupancy, fetched after the meeting a round trip)
     for (int c = threadIdx.x; c < sh.width * V; c += GN_TB)
         s_gb[c] = make_float2(a.gamma[w.span * sh.width * V + c], a.beta[w.span * sh.width * V + c]);
@@ -150,8 +162,6 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     } else {
         ok = cluster_meet<StatAcc>(sh, wk, w, as, s_pair, s_acc, &out, result, keep);
     }
-    DropKey key;
-    if constexpr (DROP) key = drop_key(rng);
     if (ok && cnt > 0) {
         Norm<T, ACT> nm[V];
         const int c0 = w.chunk * V - w.span * sh.width * V;
@@ -160,22 +170,37 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
         const long px0 = (long)w.n * sh.HW + w.p0 + w.row;
         T* y = (T*)a.y + px0 * a.ldy + w.chunk * V;
         const T* res = (const T*)a.res + px0 * a.ldres + w.chunk * V;
+        auto put = [&](int r, const Raw<T, V>* other) {
+            float f[V];
+            d[r].get(f);
+            finish<T, V, ACT>(f, nm);
+            if constexpr (DROP) keep_mask.apply(r * V, rng.scale, f);
+            if (other) {
+                float o[V];
+                other->get(o);
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (r < cnt) {
-                float f[V];
-                d[r].get(f);
-                finish<T, V, ACT>(f, nm);
-                if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)(px0 + r * sh.rows) * sh.C + w.chunk * V, f);
-                if (a.res) {
-                    float o[V];
-                    load_v<T, V>(res + (long)r * sh.rows * a.ldres, o);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) f[i] += o[i];
-                }
-                store_v<T, V>(y + (long)r * sh.rows * a.ldy, f);
-                if constexpr (V == 1 && DROP) __builtin_amdgcn_sched_barrier(0);      // (registers: not every element's generator at once)
+                for (int i = 0; i < V; ++i) f[i] += o[i];
             }
+            store_v<T, V>(y + (long)r * sh.rows * a.ldy, f);
+        };
+        if (a.res) {      // B loads in flight (beyond the image: the thread's first pixel, not used)
+            constexpr int B = V > 1 ? 2 : 8;
+#pragma unroll
+            for (int r0 = 0; r0 < R; r0 += B) {
+                Raw<T, V> o[B];
+#pragma unroll
+                for (int k = 0; k < B; ++k) o[k].load(res + (long)(r0 + k < cnt ? r0 + k : 0) * sh.rows * a.ldres);
+#pragma unroll
+                for (int k = 0; k < B; ++k) o[k].pin();
+#pragma unroll
+                for (int k = 0; k < B; ++k)
+                    if (r0 + k < cnt) put(r0 + k, o + k);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (r < cnt) put(r, nullptr);
+        }
     }
     if (sh.nb == 1) return;
     cluster_leave<StatAcc>(sh, wk, w, as, s_acc, out, result, keep, [&](int blk, const unsigned long long* fin) {

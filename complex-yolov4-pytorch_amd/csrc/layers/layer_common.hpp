@@ -2,6 +2,13 @@
 #pragma once
 #include "common.hpp"
 
+// The value as it stands: keeps the conversion to 16 bits that follows from being merged into the multiply-add before it (one rounding
+// instead of two, where the compiler finds it: two kernels' stored values would differ in their last bit).
+__device__ __forceinline__ float rounded(float v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 // V consecutive elements as floats: V = Elem<T>::CH is one 16-byte access, V = 1 takes any stride and alignment
 template <typename T, int V>
 __device__ __forceinline__ void load_v(const T* p, float* f) {
@@ -119,16 +126,43 @@ __device__ __forceinline__ void drop_apply(const DropKey& key, int q, float scal
     const u32x4 w = drop_words(key, e >> 3);
     if constexpr (V == 8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = drop_half(w, i) >= q ? f[i] * scale : 0.f;
+        for (int i = 0; i < 8; ++i) f[i] = drop_half(w, i) >= q ? rounded(f[i] * scale) : 0.f;
     } else if constexpr (V == 4) {
         const bool up = (e >> 2) & 1;
         const u32x4 h = {up ? w[2] : w[0], up ? w[3] : w[1], 0u, 0u};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = drop_half(h, i) >= q ? f[i] * scale : 0.f;
+        for (int i = 0; i < 4; ++i) f[i] = drop_half(h, i) >= q ? rounded(f[i] * scale) : 0.f;
     } else {
-        f[0] = drop_one(w, (int)(e & 7)) >= q ? f[0] * scale : 0.f;
+        f[0] = drop_one(w, (int)(e & 7)) >= q ? rounded(f[0] * scale) : 0.f;
     }
 }
+
+// The generator's answers for n elements of a thread, a bit each (1: kept), for use later.
+template <int n>
+struct DropBits {
+    unsigned bits[(n + 31) / 32];
+    // V elements from dense index e on, which are the thread's elements at, at + 1 ...: called in ascending order
+    template <int V>
+    __device__ __forceinline__ void put(const DropKey& key, int q, unsigned long long e, int at) {
+        const u32x4 w = drop_words(key, e >> 3);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int h = V == 8 ? drop_half(w, i) : V == 4 ? drop_half((e >> 2) & 1 ? u32x4{w[2], w[3], 0u, 0u} : w, i) : drop_one(w, (int)(e & 7));
+            unsigned& b = bits[(at + i) / 32];
+            b = (at + i) % 32 ? __builtin_amdgcn_alignbit(b, (unsigned)(q - 1 - h), 31) : (unsigned)(q - 1 - h) >> 31;      // shifts the sign in
+        }
+    }
+    // f[i] = kept ? f[i] * scale : 0 for the elements at, at + 1 ... (a selection: nothing comes through from a dropped place)
+    template <int V>
+    __device__ __forceinline__ void apply(int at, float scale, float (&f)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int word = (at + i) / 32, held = n - 32 * word < 32 ? n - 32 * word : 32, bit = held - 1 - (at + i) % 32;
+            const unsigned keep = (unsigned)((int)(bits[word] << (31 - bit)) >> 31);
+            f[i] = __uint_as_float(__float_as_uint(rounded(f[i] * scale)) & keep);
+        }
+    }
+};
 
 // The selection alone, on a chunk as it is stored: what is dropped becomes zero, what is kept is to be scaled.
 template <typename T, int V>
