@@ -75,18 +75,6 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     }
     int cnt = (w.px - w.row + sh.rows - 1) / sh.rows;      // pixels of this thread
     cnt = !w.on || cnt < 0 ? 0 : cnt;
-    // the generator runs while the loads are under way
-    DropKey key;
-    DropBits<R * V> keep_mask;
-    if constexpr (DROP) {
-        key = drop_key(rng);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            keep_mask.template put<V>(key, rng.q, ((unsigned long long)((long)w.n * sh.HW + w.p0 + w.row) + r * sh.rows) * sh.C + w.chunk * V, r * V);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
     // gamma and beta wait in LDS (in registers they would cost a wave of occupancy, fetched after the meeting a round trip)
     for (int c = threadIdx.x; c < sh.width * V; c += GN_TB)
         s_gb[c] = make_float2(a.gamma[w.span * sh.width * V + c], a.beta[w.span * sh.width * V + c]);
@@ -162,6 +150,8 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     } else {
         ok = cluster_meet<StatAcc>(sh, wk, w, as, s_pair, s_acc, &out, result, keep);
     }
+    DropKey key;
+    if constexpr (DROP) key = drop_key(rng);
     if (ok && cnt > 0) {
         Norm<T, ACT> nm[V];
         const int c0 = w.chunk * V - w.span * sh.width * V;
@@ -174,7 +164,7 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
             float f[V];
             d[r].get(f);
             finish<T, V, ACT>(f, nm);
-            if constexpr (DROP) keep_mask.apply(r * V, rng.scale, f);
+            if constexpr (DROP) drop_apply<V>(key, rng.q, rng.scale, (unsigned long long)(px0 + r * sh.rows) * sh.C + w.chunk * V, f);
             if (other) {
                 float o[V];
                 other->get(o);
@@ -182,6 +172,7 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
                 for (int i = 0; i < V; ++i) f[i] += o[i];
             }
             store_v<T, V>(y + (long)r * sh.rows * a.ldy, f);
+            if constexpr (V == 1 && DROP) __builtin_amdgcn_sched_barrier(0);      // (registers: not every element's generator at once)
         };
         if (a.res) {      // B loads in flight (beyond the image: the thread's first pixel, not used)
             constexpr int B = V > 1 ? 2 : 8;

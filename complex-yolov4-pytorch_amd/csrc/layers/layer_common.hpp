@@ -137,33 +137,6 @@ __device__ __forceinline__ void drop_apply(const DropKey& key, int q, float scal
     }
 }
 
-// The generator's answers for n elements of a thread, a bit each (1: kept), for use later.
-template <int n>
-struct DropBits {
-    unsigned bits[(n + 31) / 32];
-    // V elements from dense index e on, which are the thread's elements at, at + 1 ...: called in ascending order
-    template <int V>
-    __device__ __forceinline__ void put(const DropKey& key, int q, unsigned long long e, int at) {
-        const u32x4 w = drop_words(key, e >> 3);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int h = V == 8 ? drop_half(w, i) : V == 4 ? drop_half((e >> 2) & 1 ? u32x4{w[2], w[3], 0u, 0u} : w, i) : drop_one(w, (int)(e & 7));
-            unsigned& b = bits[(at + i) / 32];
-            b = (at + i) % 32 ? __builtin_amdgcn_alignbit(b, (unsigned)(q - 1 - h), 31) : (unsigned)(q - 1 - h) >> 31;      // shifts the sign in
-        }
-    }
-    // f[i] = kept ? f[i] * scale : 0 for the elements at, at + 1 ... (a selection: nothing comes through from a dropped place)
-    template <int V>
-    __device__ __forceinline__ void apply(int at, float scale, float (&f)[V]) const {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int word = (at + i) / 32, held = n - 32 * word < 32 ? n - 32 * word : 32, bit = held - 1 - (at + i) % 32;
-            const unsigned keep = (unsigned)((int)(bits[word] << (31 - bit)) >> 31);
-            f[i] = __uint_as_float(__float_as_uint(rounded(f[i] * scale)) & keep);
-        }
-    }
-};
-
 // The selection alone, on a chunk as it is stored: what is dropped becomes zero, what is kept is to be scaled.
 template <typename T, int V>
 __device__ __forceinline__ void drop_raw(const DropKey& key, int q, unsigned long long e, Raw<T, V>& x) {
