@@ -1,5 +1,6 @@
 // Dropout over a channels-last view, mask never stored:  y = kept ? x * 65536 / (65536 - q) : 0  (or added to what y holds).
-// The gradient is the same map of dy, so one kernel serves both directions.
+// The gradient is the same map of dy, so one kernel serves both directions.  Bound: memory; the generator's ten rounds are spread over
+// eight elements and stay below it.  16 x 304 x 304 x 64 bf16 63.5 us (378 MB, 6.0 TB/s), 16 x 76 x 76 x 256 f32 28 us (189 MB, 6.7 TB/s).
 #include "layer_common.hpp"
 
 namespace {

@@ -30,7 +30,8 @@ constexpr int GN_MAX_PAIRS = 384 * 1024;
 constexpr int GN_LINE = 32, GN_SUBS = 16, GN_WORDS = GN_LINE * (1 + GN_SUBS);
 constexpr int64_t GN_COUNTER_BYTES = (int64_t)GN_MAX_CLUSTERS * GN_WORDS * 4;
 constexpr int64_t GN_ZERO_BYTES = GN_COUNTER_BYTES + (int64_t)GN_MAX_PAIRS * 8;
-constexpr int GN_ONE_STEP = 4096;            // up to this many pairs (32 KB to read for every block) a cluster meets in one step
+// up to this many pairs (32 KB to read for every block) a cluster meets in one step: 361 blocks of 8 groups in two 0 to 5 % slower
+constexpr int GN_ONE_STEP = 4096;
 
 // Chunks of V elements a thread holds at most: forward x, backward x and the 32-bit dz (half as many are built, too)
 template <int V>

@@ -6,7 +6,8 @@
 //   dx = r (gamma dz - S1 - xh S2),   S1, S2 = group means of gamma dz and gamma dz xh
 //
 // This file: the choice of kernels, the C entry points, and the general kernels -- three launches per direction: partial sums per
-// (image, pixel range, column), a fold, the element pass -- for any row stride, alignment and channel count.  The one-launch kernels
+// (image, pixel range, column), a fold, the element pass -- for any row stride, alignment and channel count (16 x 304 x 304 x 64 f16
+// backward 192 us in three launches, 170 in one and the parameter gradients'; 32 x 76 x 76 x 256 bf16 with a shortcut forward 68 and 63).  The one-launch kernels
 // are in gn_resident*.  No floating-point atomics anywhere: a call's results do not depend on scheduling.
 //
 // A block works on one image n, one span of chunk columns and one range of pixels; thread = (row = t / width, chunk = t % width).
@@ -594,10 +595,10 @@ bool plan_width(int N, long HW, int C, int G, int V, int width, int R, int polls
 
 // Blocks that hold all pixels of their columns have nobody to meet: three to four microseconds less, where there are few enough of them
 // that a block's own time is what counts (f16, 8 chunks a thread unless said otherwise):
-//   1 x 19 x 19 x 1024 forward: 4 columns, alone 6.9 us; 8 columns, two blocks to an image 10.7     64 images: 27.6 against 22.4
-//   1 x 26 x 26 x 512: 2 columns 6.9; 8 columns 10.5      16 images: 4 columns, 16 chunks 11.1; 8 columns 13.4; 2 columns 15.1
-//   1 x 13 x 13 x 1024 backward: 4 columns, 4 chunks 9.4; 8 columns 12.5      16 images: 8 columns, 8 chunks 11.7; 8 columns, two blocks 15.1
-//   16 x 38 x 38 x 256 forward: 2 columns, 16 chunks (256 blocks) 16.1; 8 columns 13.4      4 images: 9.5 and 10.4
+//   1 x 19 x 19 x 1024 forward: 4 columns, alone 6.8 us; 8 columns, two blocks to an image 10.6     64 images: 27.0 against 20.3
+//   1 x 26 x 26 x 512: 2 columns 7.1; 8 columns 10.3      16 images: 4 columns, 16 chunks 8.9; 8 columns 12.5; 2 columns 16.6
+//   1 x 13 x 13 x 1024 backward: 4 columns, 4 chunks 9.5; 8 columns 12.5      16 images: 8 columns, 8 chunks 11.3; 8 columns, two blocks 14.5
+//   16 x 38 x 38 x 256 forward: 2 columns, 16 chunks (256 blocks) 19.5; 8 columns 12.4      4 images: 9.7 and 10.3
 // With a compute unit for each: as many blocks as there are compute units for, of four columns and more, or of two (up to 128 blocks).  With
 // more blocks than that: of four columns and more (backward, which reads twice as much: eight), the fewest first.
 bool plan_alone(int N, long HW, int C, int G, int V, bool bwd, int unit, int polls, ResPlan& p) {
@@ -618,10 +619,10 @@ bool plan_alone(int N, long HW, int C, int G, int V, bool bwd, int unit, int pol
 }
 
 // Columns of a block: the number nearest to eight (one 128-byte line a pixel) that cuts the row into equal spans of whole groups: narrow
-// spans make small clusters, and a narrower one splits cache lines.  16 x 76 x 76 x 256 f16 forward: 4 columns 29.2 us, 8: 24.8, 16: 24.7,
-// 32: 25.6; backward 52.9, 44.2, 44.0, 49.0; 16 x 38 x 38 x 512 f16 backward with 64: 30.8, 8: 26.9.
+// spans make small clusters, and a narrower one splits cache lines.  16 x 76 x 76 x 256 f16 forward: 4 columns 28.2 us, 8: 22.5, 16: 22.9,
+// 32: 23.4; backward 48.0, 37.6, 38.6, 42.7; 16 x 38 x 38 x 512 f16 backward with 64: 28.4, 8: 23.8.
 // Chunks of a thread: 16 (backward 8: x and the 32-bit dz), half of that where fewer than 512 blocks would be left for 256 compute units:
-// 16 x 38 x 38 x 512 f16 forward (384 blocks at 16) 19.0 us with 16, 16.5 with 8; 16 x 76 x 76 x 256 f16 (768) 24.8 with 16, 28.8 with 8.
+// 16 x 38 x 38 x 512 f16 forward (384 blocks at 16) 16.4 us with 16, 14.7 with 8; 16 x 76 x 76 x 256 f16 (768) 22.5 with 16, 27.1 with 8.
 // Element by element (rows that do not start on 16 bytes): the same in 64 columns and twice, backward four times, as many elements as there
 // would be chunks.  Up to 2048 blocks -- as many as fit at a time, about: 16 x 38 x 38 x 255 f32 forward (720 blocks) 21.6 us, three
 // launches 30.8; 16 x 76 x 76 x 255 f16 (2900 blocks) 55 and 38.

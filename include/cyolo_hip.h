@@ -322,7 +322,7 @@ int cy_bn_act_bwd_apply(const void* x, int ldx, const void* dy, int lddy, void* 
  *   y = res + drop(act(gamma[c] * (x - mean) * r + beta[c]))
  * The same function in training and in eval mode; stats (may be NULL: eval) receives (mean, r) as float [N][groups][2], 8-byte
  * aligned, for the backward pass.  res may be NULL.  Any C divisible by groups, any row strides >= C, any element-aligned pointer
- * (rows that all start on 16 bytes take the fast kernels).  y may be x (every element is read before it is written by the same
+ * (rows that all start on 16 bytes are moved 16 bytes at a time).  y may be x (every element is read before it is written by the same
  * thread); no other overlap.  N = 0 or HW = 0: nothing to do.
  * Dropout (see cy_dropout): q > 0 drops with probability q / 65536, rng / id as there; element index = ((n * HW + pixel) * C + c).
  * ws: cy_gn_workspace() bytes, 8-byte aligned, ZEROED ONCE by the caller; calls of any shape may share one that is large enough for
@@ -340,10 +340,11 @@ int cy_gn_act_bwd(const void* x, int ldx, const void* dy, int lddy, void* dx, in
                   void* ws, int64_t ws_bytes, cy_stream_t s);
 /* Bytes of ws for either call. */
 int64_t cy_gn_workspace(int N, int64_t HW, int C, int groups, int dtype);
-/* Test / tool switch, not used on the step path.  mode 0: the three-launch kernels always, 1: default (one launch where an image's rows
- * start on 16 bytes and its blocks can meet); polls: how often a block of the one-launch kernels looks for the others before it leaves
- * its pixels to the last of them (-1: default; 0: never waits); width / chunks > 0: 16-byte columns of a block / held by a thread where
- * the shape allows (0: own policy).  A workspace is sized for the setting it was asked under. */
+/* Test / tool switch, not used on the step path.  mode 0: the three-launch kernels always, 1: default (one launch where an image's
+ * blocks can meet); polls: how often a block of the one-launch kernels looks for the others before it leaves its pixels to the last of
+ * them (-1: default; 0: never waits); width > 0: columns of a block where the shape allows (of 16 bytes, or of one element where rows do
+ * not start on 16 bytes); chunks 16 / 8: as much as a thread can hold / half of it (0: own policy).  A workspace is sized for the setting
+ * it was asked under. */
 int cy_gn_config(int mode, int polls, int width, int chunks);
 
 /* Dropout over a view of M pixels x C channels, the mask never stored:
