@@ -49,22 +49,42 @@ __device__ __forceinline__ float gn_dx(const Norm<T, ACT>& nm, float2 k, float x
 
 // ---- activations -------------------------------------------------------------------------------------------------------------
 // mish(z) = z tanh(log(1 + e^z)).  With n = e^z, w = n (n + 2): tanh = w / (w + 2).  FAST (16-bit storage): hardware exponential and
-// reciprocal, 1 - 2 e each; the exponent is clamped where w / (w + 2) is 1 in 32 bits and w still finite, so no value needs a branch.
-// Derivative: with q = 2 / (w + 2) = 1 - tanh it is (1 - q) + z q^2 (w - n): one exponential, one reciprocal.
+// reciprocal, 1 - 2 e each.  The exponent is cut at 20, where w / (w + 2) is 1 in 32 bits and w finite, so no value needs a branch.
+// Derivative: with q = 2 / (w + 2) = 1 - tanh it is (1 - q) + z q^2 (w - n): one exponential, one reciprocal.  Its second term takes the
+// cut z, too: q no longer falls beyond 20, and z q^2 (w - n) would grow again from 10^16 on.  (The cut lets a NaN through.)
 // (No contraction is left to the compiler anywhere in this file: a value comes out the same wherever it is computed, by the block that
 // holds it or by the one that finishes for it.)
-constexpr float LOG2E = 1.44269504088896341f;
+//
+// 32 bits: e^z = 2^h (1 + l ln 2) with h + l = z log2(e) in two words; 1 / a by the hardware's reciprocal and one Newton step (a >= 2,
+// finite).  Within 2 e and 1 e, in 16 issue slots less per element than the library's exponential and an IEEE division:
+// 16 x 38 x 38 x 512 f32 backward 38.5 -> 34.1 us, forward 26.5 -> 22.2.
+constexpr float LOG2E = 1.44269504088896341f, LOG2E_REST = (float)(1.4426950408889634074 - (double)LOG2E), LN2 = 0.69314718055994531f;
 template <bool FAST>
-__device__ __forceinline__ float gn_exp(float z) {      // e^z, at most 2^30
-    return FAST ? __builtin_amdgcn_exp2f(fminf(z * LOG2E, 30.f)) : expf(fminf(z, 20.f));
+__device__ __forceinline__ float gn_cut(float z) {
+    z = __builtin_elementwise_minimum(z, 20.f);
+    return FAST ? z : __builtin_elementwise_maximum(z, -120.f);      // (2^h, which is 0 below 2^-126, is 0 there; the residual finite)
+}
+template <bool FAST>
+__device__ __forceinline__ float gn_exp(float z) {      // e^z of a cut z
+#pragma clang fp contract(off)
+    const float h = z * LOG2E, n = __builtin_amdgcn_exp2f(h);
+    if constexpr (FAST) return n;
+    const float l = fmaf(z, LOG2E_REST, fmaf(z, LOG2E, -h));
+    return fmaf(n, l * LN2, n);
+}
+template <bool FAST>
+__device__ __forceinline__ float gn_rcp(float a) {
+#pragma clang fp contract(off)
+    const float r = __builtin_amdgcn_rcpf(a);
+    return FAST ? r : fmaf(fmaf(-a, r, 1.f), r, r);
 }
 template <int ACT, bool FAST>
 __device__ __forceinline__ float gn_act(float z) {
 #pragma clang fp contract(off)
     if constexpr (ACT == CY_ACT_MISH) {
-        const float n = gn_exp<FAST>(z);
+        const float n = gn_exp<FAST>(gn_cut<FAST>(z));
         const float w = n * (n + 2.f);
-        return z * (FAST ? w * __builtin_amdgcn_rcpf(w + 2.f) : w / (w + 2.f));
+        return z * (w * gn_rcp<FAST>(w + 2.f));
     }
     return ACT == CY_ACT_LEAKY && !(z > 0.f) ? 0.1f * z : z;
 }
@@ -72,14 +92,14 @@ template <int ACT, bool FAST>
 __device__ __forceinline__ float gn_act_grad(float z) {
 #pragma clang fp contract(off)
     if constexpr (ACT == CY_ACT_MISH) {
+        z = gn_cut<FAST>(z);
         const float n = gn_exp<FAST>(z);
         if constexpr (FAST) {      // z q^2 (w - n) = z (n q) (n q + q)
-            const float q = __builtin_amdgcn_rcpf(fmaf(n, fmaf(n, 0.5f, 1.f), 1.f)), t = n * q;
+            const float q = gn_rcp<true>(fmaf(n, fmaf(n, 0.5f, 1.f), 1.f)), t = n * q;
             return fmaf(z * t, t + q, 1.f - q);
         }
-        const float w = n * (n + 2.f);
-        const float t = w / (w + 2.f), q = 2.f / (w + 2.f);
-        return fmaf(z * (w - n), q * q, t);      // (32 bits: tanh by itself, 1 - q cancels for large negative z)
+        const float w = n * (n + 2.f), i = gn_rcp<false>(w + 2.f), q = 2.f * i;
+        return fmaf(z * (w - n), q * q, w * i);      // (32 bits: tanh by itself, 1 - q cancels for large negative z)
     }
     return ACT == CY_ACT_LEAKY && !(z > 0.f) ? 0.1f : 1.f;
 }

@@ -285,6 +285,27 @@ def test_non_finite_values_stay_in_their_group():
     assert not bool(gg[:, 8:24].isnan().any()) and bool(gg[:, :8].isnan().all()) and bool(gg[:, 24:].isnan().all())
 
 
+@pytest.mark.parametrize('dt', [CY_F16, CY_BF16, CY_F32], ids=['f16', 'bf16', 'f32'])
+def test_mish_far_out(dt):
+    """Values whose exponential over- or underflows: mish(z) is z above and -0 below, the derivative 1 and 0.  A hardware exponential below
+    2^-126 is 0 (it has no subnormals): mish, z e^z there, is then off by at most |z| 2^-126, which no z below -87.3 makes more than
+    120 x 2^-126 of (e^z halves with every 0.7)."""
+    z = torch.tensor([0.0, -1e-6, 20.5, -20.5, 88.0, -88.0, 104.0, -104.0, 3e4, -3e4] + ([1e20, -1e20, 3e38, -3e38] if dt != CY_F16 else [6e4, -6e4]))
+    C = z.numel()
+    x = torch.tensor([[1.0], [-1.0]]).repeat(1, C)[None].to(ops.torch_dtype(dt))      # xh = +-1 / sqrt(1 + eps) in every channel
+    dy = torch.ones(1, 2, C).to(ops.torch_dtype(dt))
+    xs, ys, dys, dxs = (Strided(1, 2, 1, C, dt, fill=f) for f in (x, x, dy, dy))
+    stats, ws, gg = torch.empty(1, C, 2, device=DEV), _workspace(1, 2, 1, C, C, dt), torch.empty(2, C, device=DEV)
+    ga, be = torch.zeros(C, device=DEV), z.to(DEV)                                     # gamma = 0: z is beta
+    ops.gn_act_fwd(xs.view, ys.view, None, ga, be, C, EPS, 2, stats, ws)
+    zd = z.double()
+    want = ref.act(zd, 2)[None, None].expand(1, 2, C)
+    _close(ys.get(), want, _stored(want, dt) + 16 * E * want.abs() + 120 * 2.0 ** -126, 'y')
+    ops.gn_act_bwd(xs.view, dys.view, dxs.view, None, False, ga, be, stats, C, 2, gg[0], gg[1], 1.0, False, ws)
+    slope = ref.act_grad(zd.clamp(-700, 700), 2)
+    _close(gg[1].cpu(), 2 * slope, 16 * E * (slope.abs() + zd.abs().clamp(max=100) * (zd < 0)) + 16 * E, 'sum of the derivative')
+
+
 def test_everything_dropped():
     N, H, W, C, G = 2, 5, 7, 32, 8
     x, dy, res, gamma, beta = _problem((N, H, W, C, G, 0, 0), CY_BF16, 4)
