@@ -212,20 +212,20 @@ __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResSha
     });
 }
 
-// ggamma / gbeta from the blocks' channel sums chan[row][C][2], in double: eight channels by 128 row lanes, each lane's rows in order,
-// then the lanes in order.  Many rows are cut into gridDim.y slices: the last of them to come adds the slices' sums in order (through
+// ggamma / gbeta from the blocks' channel sums chan[row][C][2], in double: eight channels by up to 128 row lanes, each lane's rows in
+// order, then the lanes in order.  Many rows are cut into gridDim.y slices: the last of them to come adds the slices' sums in order (through
 // the cache behind the XCDs, like the meetings; the counter is zero again afterwards).  5776 rows of 64 channels: 18 us in one slice, 6.6 in sixteen.
 __global__ void __launch_bounds__(1024) gn_param_grad_kernel(const float* chan, long rows, int C, float* ggamma, float* gbeta,
                                                             float gscale, int accumulate, unsigned* counters, double* part) {
     __shared__ double s_a[128][9], s_b[128][9];
     __shared__ bool s_last;
-    const int k = threadIdx.x & 7, c = blockIdx.x * 8 + k, l = threadIdx.x >> 3, slices = gridDim.y;
+    const int k = threadIdx.x & 7, c = blockIdx.x * 8 + k, l = threadIdx.x >> 3, lanes = blockDim.x >> 3, slices = gridDim.y;
     const long per = (rows + slices - 1) / slices, r1 = (blockIdx.y + 1) * per;
     double a = 0.0, b = 0.0;
     if (c < C) {
         const float2* src = reinterpret_cast<const float2*>(chan) + c;
 #pragma unroll 8
-        for (long r = blockIdx.y * per + l; r < (r1 < rows ? r1 : rows); r += 128) {
+        for (long r = blockIdx.y * per + l; r < (r1 < rows ? r1 : rows); r += lanes) {
             const float2 v = src[r * C];
             a += (double)v.x;
             b += (double)v.y;
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(1024) gn_param_grad_kernel(const float* chan, 
     s_a[l][k] = a;
     s_b[l][k] = b;
     __syncthreads();
-    for (int h = 64; h > 0; h >>= 1) {
+    for (int h = lanes >> 1; h > 0; h >>= 1) {
         if (l < h) {
             s_a[l][k] += s_a[l + h][k];
             s_b[l][k] += s_b[l + h][k];
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(1024) gn_param_grad_kernel(const float* chan, 
         }
         __syncthreads();
         if (!s_last) return;
-        for (int t = threadIdx.x; t < slices * 16; t += 1024)      // (all at once: sixteen round trips would cost what the slices save)
+        for (int t = threadIdx.x; t < slices * 16; t += blockDim.x)      // (all at once: sixteen round trips would cost what the slices save)
             (l & 1 ? s_b : s_a)[t >> 4][k] = __longlong_as_double(__hip_atomic_load(mine + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
         __syncthreads();
         if (l == 0)
@@ -284,8 +284,10 @@ int launch(const ResPlan& p, const ResBwd& a, const ResWork& wk, const DropRng& 
     CY_LAUNCH_CHECK();
     if (a.ggamma || a.gbeta) {
         const long rows = (long)p.sh.N * p.sh.nb;
+        int lanes = 8;
+        while (lanes < 128 && lanes < rows) lanes *= 2;
         const int blocks = (p.sh.C + 7) / 8, slices = blocks > GN_MAX_CLUSTERS ? 1 : gn_param_slices(rows);
-        hipLaunchKernelGGL(gn_param_grad_kernel, dim3(blocks, slices), dim3(1024), 0, s, wk.chan, rows, p.sh.C, a.ggamma, a.gbeta, a.gscale,
+        hipLaunchKernelGGL(gn_param_grad_kernel, dim3(blocks, slices), dim3(8 * lanes), 0, s, wk.chan, rows, p.sh.C, a.ggamma, a.gbeta, a.gscale,
                            a.accumulate, wk.counters, wk.part);
         CY_LAUNCH_CHECK();
     }
