@@ -113,17 +113,20 @@ __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResSha
     }
     if (threadIdx.x == w.row * sh.width) s_n[w.row] = n;
     __syncthreads();
-    {      // the block's (mean, centred sum of squares) of every group: weighted mean first, then the squares about it
+    {      // the block's (mean, centred sum of squares) of every group: weighted mean first, then the squares about it.  The mean is summed as
+           // distances from the first thread's: a weighted sum of the means themselves would be off by many 2^-24 of a large mean, and its
+           // square, beside a small eps, is a variance that is not there (60000 in every place of a group: r = 240 for 316).
         const int per = gn_cols<V>(sh.Cg), rw = sh.width * A, E = sh.rows * per;
         const int L = lanes_for(sh.gps), l = threadIdx.x & (L - 1);
         const float total = 1.f / ((float)w.px * sh.Cg);
         for (int g = threadIdx.x / L; g < sh.gps; g += GN_TB / L) {
+            const float first = s_m[g * per];
             float sum = 0.f, m2 = 0.f;
             for (int e = l; e < E; e += L) {
                 const int r = per == 1 ? e : e / per;
-                sum += s_n[r] * s_m[r * rw + g * per + e - r * per];
+                sum += s_n[r] * (s_m[r * rw + g * per + e - r * per] - first);
             }
-            const float mean = lanes_sum(sum, L) * total;
+            const float mean = first + lanes_sum(sum, L) * total;
             for (int e = l; e < E; e += L) {
                 const int r = per == 1 ? e : e / per, at = r * rw + g * per + e - r * per;
                 const float t = s_m[at] - mean;
