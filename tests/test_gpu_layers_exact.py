@@ -1,5 +1,5 @@
-"""Group norm + activation where the result is known to the last bits.  e = 2^-24 is half a step of float32; storage adds half a step of its
-type."""
+"""Group norm + activation where the result is known to the last bits: groups of one value, and values a few steps of the type apart beside a
+large mean.  e = 2^-24 is half a step of float32; storage adds half a step of its type."""
 import pytest
 import torch
 
@@ -7,9 +7,11 @@ pytestmark = pytest.mark.gpu
 
 import complex_yolov4_pytorch_amd.ops as ops  # noqa: E402
 from complex_yolov4_pytorch_amd.ops import CY_BF16, CY_F16, CY_F32  # noqa: E402
-from tests.test_gpu_layers import DEV, E, EPS, Strided, _close, _gen, _workspace, kernels  # noqa: E402, F401
+from oracle import layers_ref as ref  # noqa: E402
+from tests.test_gpu_layers import DEV, E, EPS, Strided, _close, _gen, _stored, _workspace, kernels  # noqa: E402, F401
 
 TYPES = pytest.mark.parametrize('dt', [CY_F16, CY_BF16, CY_F32], ids=['f16', 'bf16', 'f32'])
+ACTS = pytest.mark.parametrize('act', [0, 1, 2], ids=['linear', 'leaky', 'mish'])
 SHAPES = pytest.mark.parametrize('shape', [(2, 40, 41, 64, 8), (1, 50, 50, 30, 5), (2, 13, 17, 64, 16), (1, 19, 19, 96, 3)],
                                  ids=['rows16', 'ragged', 'narrow', 'wide'])
 R = 1 / (EPS ** 0.5)
@@ -37,3 +39,53 @@ def test_statistics_of_groups_of_one_value(shape, dt, kernels):  # noqa: F811
     ops.gn_act_fwd(xs.view, ys.view, None, torch.ones(C, device=DEV), torch.zeros(C, device=DEV), G, EPS, 0, stats, _workspace(N, H, W, C, G, dt))
     assert torch.equal(stats[..., 0].cpu(), v.float())
     _close(stats[..., 1].cpu(), torch.full((N, G), R, dtype=torch.float64), torch.full((N, G), 4 * E * R, dtype=torch.float64), 'r')
+
+
+@SHAPES
+@ACTS
+@TYPES
+def test_groups_of_one_value(shape, dt, act, kernels):  # noqa: F811
+    """A dead group: x - mean is 0, so z is beta and what is left is the activation (an exponential and a reciprocal at 1 - 2 e each, five
+    operations: 16 e) and storage, however large the value beside the deviation of sqrt(eps)."""
+    N, H, W, C, G = shape
+    t = ops.torch_dtype(dt)
+    _, x = _one_value_groups(N, H * W, C, G, t)
+    gamma, beta = 1 + 0.3 * torch.randn(C, generator=_gen(2)), 0.3 * torch.randn(C, generator=_gen(3))
+    dy = torch.randn(N, H * W, C, generator=_gen(4)).to(t)
+    xs, ys, dys, dxs = Strided(N, H, W, C, dt, fill=x), Strided(N, H, W, C, dt), Strided(N, H, W, C, dt, fill=dy), Strided(N, H, W, C, dt)
+    stats, ws, gg = torch.empty(N, G, 2, device=DEV), _workspace(N, H, W, C, G, dt), torch.empty(2, C, device=DEV)
+    ga, be = gamma.to(DEV), beta.to(DEV)
+    ops.gn_act_fwd(xs.view, ys.view, None, ga, be, G, EPS, act, stats, ws)
+    want = ref.act(beta.double(), act).expand(N, H * W, C)
+    _close(ys.get(), want, _stored(want, dt) + 16 * E * beta.double().abs(), 'y')
+    # gradient: xh is 0.  A block's sum takes at most 64 additions in a row (this file's sizes), the rest is in double
+    ops.gn_act_bwd(xs.view, dys.view, dxs.view, None, False, ga, be, stats, G, act, gg[0], gg[1], 1.0, False, ws)
+    assert float(gg[0].abs().max()) == 0
+    slope = ref.act_grad(beta.double(), act)
+    dz = dy.double() * slope
+    dze = 16 * E * dy.double().abs() * (slope.abs() + beta.double().abs() * (act == 2))
+    _close(gg[1].cpu(), dz.sum((0, 1)), (dze + 64 * E * dz.abs()).sum((0, 1)), 'gbeta')
+    grp = lambda a: a.reshape(N, H * W, G, -1)      # noqa: E731
+    h, he = grp(dz * gamma.double()), grp(dze * gamma.double().abs())
+    dx = R * (h - h.mean((1, 3), keepdim=True))
+    tol = R * (he + he.mean((1, 3), keepdim=True) + 80 * E * (h.abs() + h.abs().mean((1, 3), keepdim=True)))
+    _close(dxs.get(), dx.reshape(N, H * W, C), tol.reshape(N, H * W, C) + _stored(dx.reshape(N, H * W, C), dt), 'dx')
+
+
+@SHAPES
+@ACTS
+@TYPES
+def test_outputs_beside_a_large_mean(shape, dt, act, kernels):  # noqa: F811
+    """Values up to seven steps of the type apart at 1024.  The mean is a float32 number: e |mean| of its own rounding and as much again from
+    the means of blocks; x - mean takes e of the distance, the rest is as everywhere (16 e of the terms)."""
+    N, H, W, C, G = shape
+    step = {CY_F16: 2.0 ** -10, CY_BF16: 2.0 ** -7, CY_F32: 2.0 ** -23}[dt] * 1024
+    x = (1024 + step * torch.randint(0, 8, (N, H * W, C), generator=_gen(5)).double()).to(ops.torch_dtype(dt))
+    gamma, beta = 1 + 0.3 * torch.randn(C, generator=_gen(2)), 0.3 * torch.randn(C, generator=_gen(3))
+    xs, ys = Strided(N, H, W, C, dt, fill=x), Strided(N, H, W, C, dt)
+    ops.gn_act_fwd(xs.view, ys.view, None, gamma.to(DEV), beta.to(DEV), G, EPS, act, None, _workspace(N, H, W, C, G, dt))
+    want, n = ref.gn_act(x, gamma, beta, G, EPS, act)
+    per_c = lambda t: t.repeat_interleave(C // G, -1)[:, None, :]      # noqa: E731
+    xe = 2 * E * per_c(n['mean'].abs() * n['rstd']) + (64 + 512) * E * n['xh'].abs()      # (r: 512 e, as the statistics' own test has it)
+    ze = xe * gamma.double().abs() + 16 * E * ((n['xh'] * gamma.double()).abs() + beta.double().abs())
+    _close(ys.get(), want, _stored(want, dt) + 1.1 * ze + 16 * E * want.abs(), 'y')
