@@ -1,5 +1,5 @@
-"""Group norm + activation where the result is known to the last bits: groups of one value, and values a few steps of the type apart beside a
-large mean.  e = 2^-24 is half a step of float32; storage adds half a step of its type."""
+"""Group norm + activation where the result is known to the last bits: groups of one value, values a few steps of the type apart beside a
+large mean, and the derivative of mish far below zero.  e = 2^-24 is half a step of float32; storage adds half a step of its type."""
 import pytest
 import torch
 
@@ -89,3 +89,31 @@ def test_outputs_beside_a_large_mean(shape, dt, act, kernels):  # noqa: F811
     xe = 2 * E * per_c(n['mean'].abs() * n['rstd']) + (64 + 512) * E * n['xh'].abs()      # (r: 512 e, as the statistics' own test has it)
     ze = xe * gamma.double().abs() + 16 * E * ((n['xh'] * gamma.double()).abs() + beta.double().abs())
     _close(ys.get(), want, _stored(want, dt) + 1.1 * ze + 16 * E * want.abs(), 'y')
+
+
+@TYPES
+def test_mish_derivative_below_zero(dt, kernels):  # noqa: F811
+    """gamma = 0 makes z = beta.  mish' = tanh s + z (1 - tanh^2 s) sigmoid(z), s = log(1 + e^z): far below zero both terms are e^z times a
+    small power of z and of one sign, so nothing may cancel.  e^z: the exponent z log2(e) is rounded twice (2 |z| e of e^z), an
+    exponential and a reciprocal at 2 e, eight operations: (2 |z| + 16) e of the two terms' sum.  The hardware's exponential is 0
+    below 2^-126."""
+    z = torch.cat([torch.linspace(-20, 3, 93), torch.linspace(-110, -20.5, 35)])
+    C, HW = z.numel(), 6
+    sign = torch.tensor([1.0, -1.0] * 3)
+    x = sign[None, :, None].repeat(1, 1, C).to(ops.torch_dtype(dt))                         # xh = +-1 / sqrt(1 + eps) in every channel
+    dy = torch.tensor([1.0, -0.5] * 3)[None, :, None].repeat(1, 1, C).to(ops.torch_dtype(dt))
+    xs, dys, dxs = Strided(1, HW, 1, C, dt, fill=x), Strided(1, HW, 1, C, dt, fill=dy), Strided(1, HW, 1, C, dt)
+    stats, ws, gg = torch.empty(1, C, 2, device=DEV), _workspace(1, HW, 1, C, C, dt), torch.empty(2, C, device=DEV)
+    ga, be = torch.zeros(C, device=DEV), z.to(DEV)
+    ops.gn_act_fwd(xs.view, dxs.view, None, ga, be, C, EPS, 2, stats, ws)
+    ops.gn_act_bwd(xs.view, dys.view, dxs.view, None, False, ga, be, stats, C, 2, gg[0], gg[1], 1.0, False, ws)
+    zd = z.double()
+    n = zd.exp()
+    w = n * (n + 2)
+    t = w / (w + 2)
+    second = zd * (4 * (w + 1) / (w + 2) ** 2) * torch.sigmoid(zd)      # (1 - tanh^2 = 4 (w + 1) / (w + 2)^2)
+    slope = t + second
+    xh = 1 / (1 + EPS) ** 0.5
+    tol = (2 * zd.abs() + 16) * E * (t + second.abs()) + 120 * 2.0 ** -126
+    _close(gg[1].cpu(), 1.5 * slope, 3 * 1.5 * tol + 8 * E * slope.abs(), 'gbeta')
+    _close(gg[0].cpu(), 4.5 * slope * xh, 4.5 * (tol + 8 * E * slope.abs()), 'ggamma')
