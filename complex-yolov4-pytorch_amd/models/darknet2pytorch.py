@@ -107,7 +107,8 @@ class Darknet(nn.Module):
         self.loss = self.models[len(self.models) - 1]
         self.header = torch.IntTensor([0, 0, 0, 0])
         self.seen = 0
-        self._drop_seed, self._drop_step, self._drop_dev = None, 0, None      # [dropout]: see seed_dropout
+        self._drop_dev = None            # [dropout]: (seed, step) on the device, see seed_dropout
+        self.seed_dropout(None)
         self.cpu_outputs = True          # targets=None returns a CPU tensor like the reference (:228)
         import collections
         self._plans, self._engines = {}, collections.OrderedDict()      # engines in least-recently-used order (see _engine_for)
@@ -166,29 +167,44 @@ class Darknet(nn.Module):
         stepping without a training forward of this module).  Only needed with ``static_eval_weights = True``."""
         self._weights_epoch += 1
 
-    def seed_dropout(self, seed, step=0):
-        """Seed of the [dropout] masks (default: torch.initial_seed(), with the rank mixed in under torch.distributed: ranks that
-        share a seed would drop the same places of their different images) and the number of training forwards done so far:
-        ``seed_dropout(*model.dropout_position())`` after a resume continues the sequence."""
-        self._drop_seed, self._drop_step = int(seed), int(step)
+    def seed_dropout(self, seed, step=0, per_rank=False):
+        """Seed of the [dropout] masks and the number of training forwards done so far.  ``seed`` None (the state of a new model):
+        torch.initial_seed() at the first training forward, per rank.  ``per_rank`` mixes the rank into the seed under
+        torch.distributed: ranks that share a seed drop the same places of their different images."""
+        self._drop_base, self._drop_step, self._drop_per_rank = None if seed is None else int(seed), int(step), bool(per_rank)
         if self._drop_dev is not None:      # (in place: a captured step reads and advances this tensor)
-            self._drop_dev.copy_(ops.dropout_state(seed, self._drop_dev.device, step))
+            self._drop_dev.copy_(ops.dropout_state(self._first_seed(), self._drop_dev.device, step))
 
     def dropout_position(self):
-        """(seed, training forwards done) of the dropout masks; reads the device counter."""
+        """(seed of this rank, training forwards done) of the dropout masks; reads the device counter.
+        ``seed_dropout(*position)`` continues the sequence in a process of its own or on the same rank; every rank of a resumed
+        run takes ``dropout_state_dict``."""
         if self._drop_dev is not None:
             self._drop_step = int(self._drop_dev[1])
-        return self._drop_seed, self._drop_step
+        return self._rank_seed(), self._drop_step
+
+    def dropout_state_dict(self):
+        """What a resumed run passes to ``seed_dropout(**state)``, the same on every rank (get_saved_state carries it)."""
+        return {'seed': self._drop_base, 'step': self.dropout_position()[1], 'per_rank': self._drop_per_rank}
+
+    def has_dropout(self):
+        return any(b['type'] == 'dropout' and float(b.get('probability', 0.5)) > 0 for b in self.blocks[1:])
+
+    def _rank_seed(self):
+        seed = self._drop_base
+        if seed is not None and self._drop_per_rank and torch.distributed.is_available() and torch.distributed.is_initialized():
+            seed = (seed + torch.distributed.get_rank() * 0x9E3779B97F4A7C15) % (1 << 64)
+        return seed
+
+    def _first_seed(self):
+        if self._drop_base is None:
+            self._drop_base, self._drop_per_rank = torch.initial_seed(), True
+        return self._rank_seed()
 
     def _dropout_state(self, device):
         if self._drop_dev is None or self._drop_dev.device != device:
-            seed, step = self.dropout_position()
-            if seed is None:
-                seed = torch.initial_seed()
-                if torch.distributed.is_available() and torch.distributed.is_initialized():
-                    seed += torch.distributed.get_rank() * 0x9E3779B97F4A7C15
-                self._drop_seed = seed = seed % (1 << 64)
-            self._drop_dev = ops.dropout_state(seed, device, step)
+            step = self.dropout_position()[1]
+            self._drop_dev = ops.dropout_state(self._first_seed(), device, step)
         return self._drop_dev
 
     def load_state_dict(self, *args, **kwargs):

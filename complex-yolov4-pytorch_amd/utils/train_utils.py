@@ -39,10 +39,13 @@ def create_optimizer(configs, model):
 
 def get_saved_state(model, optimizer, lr_scheduler, epoch, configs):
     """(model state dict, {'epoch', 'configs', 'optimizer', 'lr_scheduler'}) as reference train_utils.py:80-93.  The model
-    state dict holds the fp32 master parameters under the reference's keys, so the checkpoint loads into the reference."""
+    state dict holds the fp32 master parameters under the reference's keys, so the checkpoint loads into the reference.  A model with
+    [dropout] blocks adds 'dropout', the position of its masks: a resumed run calls ``model.seed_dropout(**state['dropout'])``."""
     m = model.module if hasattr(model, 'module') else model
     utils_state_dict = {'epoch': epoch, 'configs': configs, 'optimizer': copy.deepcopy(optimizer.state_dict()),
                         'lr_scheduler': copy.deepcopy(lr_scheduler.state_dict())}
+    if getattr(m, 'has_dropout', bool)():
+        utils_state_dict['dropout'] = m.dropout_state_dict()
     return m.state_dict(), utils_state_dict
 
 
