@@ -560,12 +560,13 @@ int backward(const T* x, int ldx, const T* dy, int lddy, T* dx, int lddx, T* res
 }
 
 // ---- the one-launch kernels: which calls take them ---------------------------------------------------------------------------
-// Test / tool switch (cy_gn_config)
+// Test / tool switch (cy_gn_config), of the thread that sets it: a call of another thread keeps the kernels that its workspace was sized for
 struct Config {
     int mode, polls, width, R;
 };
 constexpr int POLLS = 1024;      // about a millisecond
-Config g_cfg = {1, POLLS, 0, 0};
+constexpr Config DEFAULTS = {1, POLLS, 0, 0};
+thread_local Config t_cfg = DEFAULTS;
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
@@ -626,8 +627,7 @@ bool plan_alone(int N, long HW, int C, int G, int V, bool bwd, int unit, int pol
 // Element by element (rows that do not start on 16 bytes): the same in 64 columns and twice, backward four times, as many elements as there
 // would be chunks.  Up to 2048 blocks -- as many as fit at a time, about: 16 x 38 x 38 x 255 f32 forward (720 blocks) 21.6 us, three
 // launches 30.8; 16 x 76 x 76 x 255 f16 (2900 blocks) 55 and 38.
-bool plan_resident(int N, long HW, int C, int G, int V, bool bwd, ResPlan& p) {
-    const Config cfg = g_cfg;
+bool plan_resident(int N, long HW, int C, int G, int V, bool bwd, ResPlan& p, const Config& cfg = t_cfg) {
     if (!cfg.mode || C % V) return false;
     const int Cg = C / G, unit = Cg / gcd(Cg, V);      // columns of the smallest span of whole groups and whole chunks
     const int cpr = C / V, units = cpr / unit, most = gn_held(V, bwd), line = columns(V);
@@ -739,17 +739,18 @@ extern "C" int64_t cy_gn_workspace(int N, int64_t HW, int C, int groups, int dty
         if (C % V) continue;
         const int64_t v = 4 * need_floats(make_shape(N, (long)HW, C, groups, V));
         if (v > most) most = v;
-        for (int bwd = 0; bwd < 2; ++bwd) {
-            ResPlan p;
-            if (plan_resident(N, (long)HW, C, groups, V, bwd != 0, p) && resident_bytes(p) > most) most = resident_bytes(p);
-        }
+        for (int bwd = 0; bwd < 2; ++bwd)
+            for (const Config& cfg : {t_cfg, DEFAULTS}) {      // (a backward pass runs in a thread of its own)
+                ResPlan p;
+                if (plan_resident(N, (long)HW, C, groups, V, bwd != 0, p, cfg) && resident_bytes(p) > most) most = resident_bytes(p);
+            }
     }
     return GN_ZERO_BYTES + most;
 }
 
 extern "C" int cy_gn_config(int mode, int polls, int width, int chunks) {
     if (mode < 0 || mode > 1 || polls < -1 || width < 0 || (chunks != 0 && chunks != 8 && chunks != 16)) return CY_ERR_ARG;
-    g_cfg = Config{mode, polls < 0 ? POLLS : polls, width, chunks};
+    t_cfg = Config{mode, polls < 0 ? POLLS : polls, width, chunks};
     return 0;
 }
 

@@ -659,7 +659,7 @@ def gn_workspace(N, H, W, C, groups, dt, device='cuda'):
 
 
 def gn_config(mode=1, polls=-1, width=0, chunks=0):
-    """Test / tool switch of the group norm kernels (cy_gn_config)."""
+    """Test / tool switch of the group norm kernels for calls of this thread (cy_gn_config)."""
     lib().call('cy_gn_config', int(mode), int(polls), int(width), int(chunks))
 
 

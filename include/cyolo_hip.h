@@ -191,7 +191,7 @@ int64_t cy_pipe_launches(void);
  * BN statistics into shared bins or the eval-mode epilogue.  CY_CONV_TILE(1) or CY_CONV_DIRECT=0 in the environment keep
  * a call on the implicit-GEMM kernels. */
 int64_t cy_direct_launches(void);
-/* Test / tool switch, not used on the step path.  mode 0: never use the pipelined kernel, 1: default (hints and the
+/* Test / tool switch of the calling thread, not used on the step path.  mode 0: never use the pipelined kernel, 1: default (hints and the
  * eval-mode epilogue select it), 2: every launch that qualifies; cap x bn (0 x 0 = policy) forces a tile capacity out of
  * {384,256,192,128} x 128 / {384,256,128} x 64 with bm_eff (0 = cap) pixels of it used; variant 0: shipped (3-stage ring,
  * LDS-transposed stores), 1: direct stores from the MFMA layout (what CY_CONV_ACCUM launches use), 2: 2-stage ring,
@@ -340,11 +340,11 @@ int cy_gn_act_bwd(const void* x, int ldx, const void* dy, int lddy, void* dx, in
                   void* ws, int64_t ws_bytes, cy_stream_t s);
 /* Bytes of ws for either call. */
 int64_t cy_gn_workspace(int N, int64_t HW, int C, int groups, int dtype);
-/* Test / tool switch, not used on the step path.  mode 0: the three-launch kernels always, 1: default (one launch where an image's
+/* Test / tool switch of the calling thread, not used on the step path.  mode 0: the three-launch kernels always, 1: default (one launch where an image's
  * blocks can meet); polls: how often a block of the one-launch kernels looks for the others before it leaves its pixels to the last of
  * them (-1: default; 0: never waits); width > 0: columns of a block where the shape allows (of 16 bytes, or of one element where rows do
  * not start on 16 bytes); chunks 16 / 8: as much as a thread can hold / half of it (0: own policy).  A workspace is sized for the setting
- * it was asked under. */
+ * it was asked under and for the default one. */
 int cy_gn_config(int mode, int polls, int width, int chunks);
 
 /* Dropout over a view of M pixels x C channels, the mask never stored:
