@@ -754,6 +754,21 @@ extern "C" int cy_gn_config(int mode, int polls, int width, int chunks) {
     return 0;
 }
 
+extern "C" int cy_gn_plan(int N, int64_t HW, int C, int groups, int dtype, int backward, int rows16, int* plan) {
+    const int V = !rows16 ? 1 : dtype == CY_F32 ? 4 : 8;
+    if (!sizes_ok(N, HW, C, groups, dtype) || N == 0 || HW == 0 || C % V || !plan) return CY_ERR_ARG;
+    ResPlan p;
+    if (plan_resident(N, (long)HW, C, groups, V, backward != 0, p)) {
+        const int out[6] = {1, p.sh.width, p.R, p.sh.nspan, p.sh.nb, p.sh.nsub};
+        for (int i = 0; i < 6; ++i) plan[i] = out[i];
+    } else {
+        const Shape sh = make_shape(N, (long)HW, C, groups, V);
+        const int out[6] = {3, sh.width, 0, sh.nspan, sh.nblk, 0};
+        for (int i = 0; i < 6; ++i) plan[i] = out[i];
+    }
+    return 0;
+}
+
 extern "C" int cy_gn_act_fwd(const void* x, int ldx, void* y, int ldy, const void* res, int ldres, int N, int64_t HW, int C,
                              int groups, const float* gamma, const float* beta, float eps, int act, int dtype, float* stats, int q,
                              const int64_t* rng, int id, void* ws, int64_t ws_bytes, cy_stream_t s) {

@@ -663,6 +663,14 @@ def gn_config(mode=1, polls=-1, width=0, chunks=0):
     lib().call('cy_gn_config', int(mode), int(polls), int(width), int(chunks))
 
 
+def gn_plan(N, H, W, C, groups, dt, backward=False, rows16=True):
+    """What a call of this shape would run (cy_gn_plan): launches, columns, chunks, spans, blocks, combiners."""
+    out = (ctypes.c_int * 6)()
+    if lib().raw('cy_gn_plan')(N, H * W, C, groups, dt, int(backward), int(rows16), out):
+        raise CyoloError('cy_gn_plan: %d channels in %d groups (N %d, %d x %d, type %r, rows16 %r)' % (C, groups, N, H, W, dt, rows16))
+    return dict(zip(('launches', 'columns', 'chunks', 'spans', 'blocks', 'combiners'), out))
+
+
 def _check_gn(who, x, gamma, beta, groups, act, ws, dev):
     if groups < 1 or x.C % groups:
         raise CyoloError('%s: %d channels do not divide into %d groups' % (who, x.C, groups))

@@ -346,6 +346,10 @@ int64_t cy_gn_workspace(int N, int64_t HW, int C, int groups, int dtype);
  * not start on 16 bytes); chunks 16 / 8: as much as a thread can hold / half of it (0: own policy).  A workspace is sized for the setting
  * it was asked under and for the default one. */
 int cy_gn_config(int mode, int polls, int width, int chunks);
+/* Test / tool query: what a call of this shape would run under the thread's setting, rows16: every row of every operand starts on 16
+ * bytes.  plan[6] = launches (1 or 3; the parameter gradients' not counted), columns of a block, chunks a thread holds (0: three
+ * launches), spans of a pixel row, blocks of an image and span, blocks that combine others' pairs (0: all meet in one step). */
+int cy_gn_plan(int N, int64_t HW, int C, int groups, int dtype, int backward, int rows16, int* plan);
 
 /* Dropout over a view of M pixels x C channels, the mask never stored:
  *   y = keep[e] ? x * 65536 / (65536 - q) : 0     (accumulate: added to what y holds)

@@ -1,0 +1,36 @@
+"""Which kernels a shape takes (ops.gn_plan), on the host.  The device tests of meetings in two steps rely on it."""
+import pytest
+
+from complex_yolov4_pytorch_amd import ops
+from complex_yolov4_pytorch_amd.ops import CY_BF16, CY_F16, CY_F32
+
+# N, H, W, C, G, type, directions in which the blocks of an image meet in two steps; the last combiner has fewer blocks than the others
+TWO_STEPS = [((1, 190, 190, 64, 32), CY_F16, (False, True)), ((1, 190, 190, 64, 32), CY_BF16, (False, True)),
+             ((1, 280, 280, 64, 32), CY_F32, (False, True)), ((2, 230, 230, 64, 32), CY_F16, (False, True))]
+
+
+@pytest.mark.parametrize('shape,dt,directions', TWO_STEPS)
+def test_shapes_that_meet_in_two_steps(shape, dt, directions):
+    for bwd in directions:
+        p = ops.gn_plan(*shape, dt, backward=bwd)
+        each = -(-p['blocks'] // p['combiners'])
+        assert p['launches'] == 1 and p['combiners'] > 1 and p['blocks'] % each
+
+
+def test_plan_of_small_and_ragged_calls():
+    assert ops.gn_plan(1, 19, 19, 1024, 32, CY_F16)['blocks'] == 1
+    assert ops.gn_plan(1, 75, 43, 30, 6, CY_F32, rows16=False)['launches'] == 1
+    assert ops.gn_plan(16, 76, 76, 255, 17, CY_F16, rows16=False)['launches'] == 3
+    ops.gn_config(mode=0)
+    try:
+        assert ops.gn_plan(1, 19, 19, 1024, 32, CY_F16)['launches'] == 3
+    finally:
+        ops.gn_config()
+
+
+@pytest.mark.parametrize('bad', [dict(N=0), dict(H=0), dict(C=30), dict(groups=3), dict(dt=7)])
+def test_refusals(bad):
+    a = dict(N=1, H=4, W=4, C=16, groups=4, dt=CY_F16)
+    a.update(bad)
+    with pytest.raises(ops.CyoloError):
+        ops.gn_plan(**a)
