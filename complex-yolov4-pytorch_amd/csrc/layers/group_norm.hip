@@ -624,9 +624,18 @@ bool plan_alone(int N, long HW, int C, int G, int V, bool bwd, int unit, int pol
 // 32: 23.4; backward 48.0, 37.6, 38.6, 42.7; 16 x 38 x 38 x 512 f16 backward with 64: 28.4, 8: 23.8.
 // Chunks of a thread: 16 (backward 8: x and the 32-bit dz), half of that where fewer than 512 blocks would be left for 256 compute units:
 // 16 x 38 x 38 x 512 f16 forward (384 blocks at 16) 16.4 us with 16, 14.7 with 8; 16 x 76 x 76 x 256 f16 (768) 22.5 with 16, 27.1 with 8.
+// Where half as many make the cluster too large, all of them: 1 x 608 x 608 x 32 f16 forward 4 columns, 16 chunks 23.2 us; three launches 31.3.
+// A large image of a small batch, too many blocks at eight columns: not less than half a line unless that is the whole row, and half a line
+// only while all blocks fit at a time (1024), else three launches (us: narrow, three launches):
+//   1 x 1216 x 1216 x 32 f16 forward  1 column of 4   204  64      1 x 608 x 608 x 64 f16 forward   4 of 8,  722 blocks   35.5  43.4
+//   1 x 1024 x 1024 x 32 f16 forward  2 of 4           80  50      1 x 400 x 400 x 64 f16 backward  4 of 8,  626 blocks   31.8  35.3
+//   1 x  608 x  608 x 64 f16 backward 2 of 8          112  58      1 x 480 x 480 x 64 f32 backward  4 of 16, 1800 blocks  63.6  56.6
+//   1 x  800 x  800 x 64 f32 backward 1 of 16         698 158      1 x 512 x 512 x 128 f16 backward 4 of 16, 2048 blocks  97.7  71.6
 // Element by element (rows that do not start on 16 bytes): the same in 64 columns and twice, backward four times, as many elements as there
 // would be chunks.  Up to 2048 blocks -- as many as fit at a time, about: 16 x 38 x 38 x 255 f32 forward (720 blocks) 21.6 us, three
-// launches 30.8; 16 x 76 x 76 x 255 f16 (2900 blocks) 55 and 38.
+// launches 30.8; 16 x 76 x 76 x 255 f16 (2900 blocks) 55 and 38.  Backward with less than half of that line: up to 1024 (1 x 608 x 608 x 30 f32,
+// 10 columns, 1389 blocks 71.6 and 52.3; 1 x 304 x 304 x 30 f32, 15 columns, 680 blocks 23.8 and 28.8).
+constexpr long AT_A_TIME = 1024;
 bool plan_resident(int N, long HW, int C, int G, int V, bool bwd, ResPlan& p, const Config& cfg = t_cfg) {
     if (!cfg.mode || C % V) return false;
     const int Cg = C / G, unit = Cg / gcd(Cg, V);      // columns of the smallest span of whole groups and whole chunks
@@ -647,13 +656,19 @@ bool plan_resident(int N, long HW, int C, int G, int V, bool bwd, ResPlan& p, co
         if (!width) return false;
         tried = best;
         if (cfg.width && cfg.width % unit == 0 && cpr % cfg.width == 0 && cfg.width <= GN_TB) width = cfg.width;
+        const bool part = width < cpr && !cfg.width;      // (of a pixel row)
+        if (part && V > 1 && 2 * width < line) continue;
         int R = cfg.R ? cfg.R * most / 16 : most;
         if (!cfg.R) {
             const long ppb = (long)most * (GN_TB / width);
             if ((long)N * (cpr / width) * ((HW + ppb - 1) / ppb) < 512) R = most / 2;
         }
-        if (plan_width(N, HW, C, G, V, width, R, cfg.polls, p)) return V > 1 || cfg.width || (long)N * p.sh.nspan * p.sh.nb <= 2048;
-        if (cfg.width) return false;
+        bool fits = plan_width(N, HW, C, G, V, width, R, cfg.polls, p);
+        if (!fits && V > 1 && !cfg.R && R < most) fits = plan_width(N, HW, C, G, V, width, most, cfg.polls, p);
+        if (!fits && cfg.width) return false;
+        const long blocks = (long)N * p.sh.nspan * p.sh.nb;
+        if (!fits || (part && width < line && blocks > AT_A_TIME && (V > 1 || (bwd && 2 * width < line)))) continue;
+        return V > 1 || cfg.width || blocks <= 2 * AT_A_TIME;
     }
 }
 

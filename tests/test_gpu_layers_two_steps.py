@@ -1,12 +1,12 @@
-"""Images whose blocks meet in two steps, in both directions, with blocks that wait and blocks that never do (the last one out then combines
-both steps by itself): against the 64-bit formulas, and the same bits either way."""
+"""Images of many blocks, and such whose blocks meet in two steps, in both directions, with blocks that wait and blocks that never do (the last one out
+then combines both steps by itself): against the 64-bit formulas, and the same bits either way."""
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 
 import complex_yolov4_pytorch_amd.ops as ops  # noqa: E402
-from complex_yolov4_pytorch_amd.ops import View  # noqa: E402
+from complex_yolov4_pytorch_amd.ops import CY_BF16, CY_F16, CY_F32, View  # noqa: E402
 from tests.test_gpu_layers import COUNTERS, DEV, EPS, NAMES, _problem, _workspace, test_many_images_blocks_and_columns as _against_the_formulas  # noqa: E402
 from tests.test_layers_plans import TWO_STEPS  # noqa: E402
 
@@ -17,6 +17,14 @@ CASES = pytest.mark.parametrize('shape,dt', [(s, dt) for s, dt, _ in TWO_STEPS],
 @pytest.mark.parametrize('config', [{}, dict(polls=0)], ids=['policy', 'nowait'])
 def test_against_the_formulas(shape, dt, config):
     _against_the_formulas((*shape, 0, 0), dt, config)
+
+
+@pytest.mark.parametrize('shape,dt', [((1, 530, 520, 32, 8), CY_F16),      # one launch with all chunks forward, three launches backward
+                                      ((1, 500, 500, 32, 8), CY_BF16),     # one launch with all chunks both ways
+                                      ((1, 400, 420, 64, 16), CY_F16)],    # half a line to a block backward
+                         ids=['530x520x32', '500x500x32', '400x420x64'])
+def test_large_images_of_a_batch_of_one(shape, dt):
+    _against_the_formulas((*shape, 0, 0), dt, {})
 
 
 @CASES

@@ -34,3 +34,25 @@ def test_refusals(bad):
     a.update(bad)
     with pytest.raises(ops.CyoloError):
         ops.gn_plan(**a)
+
+
+@pytest.mark.parametrize('dt', [CY_F16, CY_BF16, CY_F32])
+@pytest.mark.parametrize('bwd', [False, True])
+def test_one_launch_does_not_cut_pixels_into_slivers(dt, bwd):
+    """Blocks that cannot hold their pixels at the full width: three launches, not columns of less than half a 128-byte line -- each line would
+    go to four and more clusters -- and half a line only while all blocks fit on the chip at a time."""
+    v = 4 if dt == CY_F32 else 8
+    for N in (1, 2, 4, 16):
+        for side in (152, 304, 400, 480, 608, 800, 1024, 1216):
+            for C, G in ((32, 8), (64, 16), (64, 32), (128, 32), (592, 74), (1016, 127), (256, 8)):
+                p = ops.gn_plan(N, side, side, C, G, dt, backward=bwd)
+                if p['launches'] == 1 and p['spans'] > 1 and p['blocks'] > 1:
+                    assert p['columns'] >= 4 and (p['columns'] >= 8 or N * p['spans'] * p['blocks'] <= 1024), (N, side, C, G, p)
+                assert p['columns'] * p['spans'] == C // v or p['launches'] == 3
+
+
+def test_a_cluster_that_fits_with_all_chunks_keeps_its_width():
+    p = ops.gn_plan(1, 608, 608, 32, 8, CY_F16)
+    assert (p['launches'], p['columns'], p['chunks']) == (1, 4, 16)
+    p = ops.gn_plan(1, 500, 500, 32, 8, CY_F16, backward=True)
+    assert (p['launches'], p['columns'], p['chunks']) == (1, 4, 8)
