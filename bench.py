@@ -29,22 +29,17 @@ import os
 import sys
 import time
 
-# Before the HIP runtime comes up: the step uses two streams (main + weight-gradient side stream) and a third for the
-# gradient all-reduce.  HIP multiplexes streams over GPU_MAX_HW_QUEUES hardware queues (default 4); once RCCL has created
-# its own streams the three collide on ONE queue and run serialised (rocprofv3 timeline: 686 instead of 765 images/s under
-# CY_DDP_FORCE=1).  Eight queues keep them apart.  (An environment that spells out the default of four means no more by it: with RCCL
-# in the process it costs 878 -> 794 images/s.)
-os.environ.setdefault('GPU_MAX_HW_QUEUES', '8')
-if os.environ['GPU_MAX_HW_QUEUES'] == '4' and (os.environ.get('CY_DDP_FORCE') == '1' or int(os.environ.get('WORLD_SIZE', '1')) > 1):
-    os.environ['GPU_MAX_HW_QUEUES'] = '8'
+ROOT = os.path.dirname(os.path.abspath(__file__))
+sys.path.insert(0, ROOT)
+
+# Before the HIP runtime comes up: the package sets the number of hardware queues (the step uses two streams and a third for the gradient
+# all-reduce; rocprofv3 timeline under CY_DDP_FORCE=1: 686 images/s with four queues for 765).
+import complex_yolov4_pytorch_amd  # noqa: E402,F401
 # dmabuf IPC is what RCCL needs on this driver; the HSA runtime reads it when it initialises (the first HIP call), so here, not later
 os.environ.setdefault('HSA_ENABLE_IPC_MODE_LEGACY', '0')
 
-import torch
-import torch.distributed as dist
-
-ROOT = os.path.dirname(os.path.abspath(__file__))
-sys.path.insert(0, ROOT)
+import torch  # noqa: E402
+import torch.distributed as dist  # noqa: E402
 
 import complex_yolov4_pytorch_amd.ops as ops  # noqa: E402
 import complex_yolov4_pytorch_amd.synthetic as syn  # noqa: E402
