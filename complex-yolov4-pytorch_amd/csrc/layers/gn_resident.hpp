@@ -18,7 +18,8 @@
 //
 // Everything that blocks say to each other goes through agent-scope atomics (performed behind the XCDs' separate L2 caches).  A block
 // counts itself out of the cluster when its own stores have been performed (vmcnt) and it has read what it needs; the last one out
-// puts counters and pairs back to zero: a workspace starts zeroed and is left so.
+// puts counters and pairs back to zero: a workspace starts zeroed and is left so.  (One that is not -- never zeroed, or two calls at once in it
+// -- gives wrong results; the list's bounds are checked all the same, so that nothing outside the workspace is touched.)
 #pragma once
 #include "layer_common.hpp"
 
@@ -244,7 +245,8 @@ __device__ __forceinline__ bool cluster_meet(const ResShape& sh, const ResWork& 
     __syncthreads();
     if (threadIdx.x == 0) {
         if (!ok) {
-            agent_store(wk.list + (long)w.cluster * sh.nb + agent_add(cnt + 1, 1u), (unsigned)w.blk);
+            const unsigned at = agent_add(cnt + 1, 1u);      // (in a workspace that was left as it should not be this may be any number)
+            if (at < (unsigned)sh.nb) agent_store(wk.list + (long)w.cluster * sh.nb + at, (unsigned)w.blk);
             stores_done();
         }
         *out = agent_add(sh.nb <= GN_SUBS ? cnt : cnt + GN_LINE * (1 + w.blk % GN_SUBS), 1u);
@@ -288,7 +290,10 @@ __device__ __forceinline__ void cluster_leave(const ResShape& sh, const ResWork&
             keep(g, r);
         });
         stores_done();
-        for (unsigned i = 0; i < left; ++i) rest((int)agent_load(wk.list + (long)w.cluster * sh.nb + i), fin);
+        for (unsigned i = 0; i < left && i < (unsigned)sh.nb; ++i) {
+            const unsigned blk = agent_load(wk.list + (long)w.cluster * sh.nb + i);
+            if (blk < (unsigned)sh.nb) rest((int)blk, fin);
+        }
     }
     for (int i = t; i < (sh.nb + sh.nsub) * sh.gps; i += 64) __hip_atomic_store(one + i, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (t <= GN_SUBS) {
