@@ -1,6 +1,8 @@
 // Dropout over a channels-last view, mask never stored:  y = kept ? x * 65536 / (65536 - q) : 0  (or added to what y holds).
-// The gradient is the same map of dy, so one kernel serves both directions.  Bound: memory; the generator's ten rounds are spread over
-// eight elements and stay below it.  16 x 304 x 304 x 64 bf16 63.5 us (378 MB, 6.0 TB/s), 16 x 76 x 76 x 256 f32 28 us (189 MB, 6.7 TB/s).
+// The gradient is the same map of dy, so one kernel serves both directions.  Bound in 16-byte accesses (V = CH): memory; the generator's ten
+// rounds are spread over eight elements (f32: four) and stay below it.  16 x 304 x 304 x 64 bf16 63.5 us (378 MB, 6.0 TB/s), 16 x 76 x 76 x 256
+// f32 28 us (189 MB, 6.7 TB/s).  Element by element (V = 1: rows that do not start on 16 bytes): the generator, all ten rounds for every
+// element, and a division; 16 x 76 x 76 x 255 f16 71 us where 256 channels take 17.
 #include "layer_common.hpp"
 
 namespace {

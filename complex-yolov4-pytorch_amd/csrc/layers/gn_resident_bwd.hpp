@@ -31,7 +31,9 @@ struct SumAcc {
 // as stored in the registers, leaves room for four waves a SIMD in place of three and is slower all the same, since blocks of one image
 // compute at the same time: by 12 % on 16 x 304 x 304 x 64 f16, by 27 % on 16 x 76 x 76 x 256 bf16 with dropout.  14 chunks a thread and
 // two waves: 4 % faster on the former, 9 % slower on the latter.
-// Bound: memory while blocks load and store, the arithmetic and the meeting in between; 16 x 304 x 304 x 64 f16, mish: 163 us for 568 MB.
+// Bound: memory while blocks load and store, the arithmetic and the meeting in between; 16 x 304 x 304 x 64 f16, mish: 171 us for 568 MB.
+// With the shortcut's gradient added 60 us where it takes 39 without (16 x 76 x 76 x 256 bf16; 237 and 142 MB): its loads and stores follow one
+// another in front of the sums.
 template <typename T, int V, bool ONE, int ACT, bool DROP, int R>
 __global__ void __launch_bounds__(GN_TB) gn_bwd_resident_kernel(ResBwd a, ResShape sh, ResWork wk, DropRng rng) {
     constexpr int H = V < 4 ? V : 4;      // channels at a time

@@ -55,7 +55,7 @@ struct StatAcc {
 // R: chunks of V elements of x a thread holds.  A: sums a thread keeps (gn_sums).
 // Bound: memory while blocks load and store (4 waves a SIMD hold 64 MB of x on the chip); a block's life on an idle chip is 7 us of loads,
 // 1.5 of sums, 4 to 6 of meeting, 4 of activation and stores.  16 x 152 x 152 x 128 f16 leaky 40 us for 189 MB; 16 x 608 x 608 x 32 f16 mish
-// 175 us for 757 MB (361 blocks an image: three images at a time).  48 chunks a thread, two waves: 57 and 220 where 16 took 53 and 209.
+// 178 us for 757 MB (361 blocks an image: three images at a time).  48 chunks a thread, two waves: 57 and 220 where 16 took 53 and 209.
 template <typename T, int V, int A, int ACT, bool DROP, int R>
 __global__ void __launch_bounds__(GN_TB) gn_fwd_resident_kernel(ResFwd a, ResShape sh, ResWork wk, DropRng rng) {
     constexpr int PER = V / A;      // PER: channels of a chunk that share a sum

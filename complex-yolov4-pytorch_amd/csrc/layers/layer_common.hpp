@@ -128,7 +128,8 @@ __device__ __forceinline__ int drop_one(const u32x4& w, int j) {
 }
 
 // f[i] = kept ? f[i] * scale : 0 for the V elements from dense element index e on.  A selection, not a product: what is in a dropped
-// place (a NaN too) does not come through.  e is a multiple of V.
+// place (a NaN too) does not come through.  e is a multiple of V.  V = 1 runs the ten rounds for one half-word of eight (group norm +
+// dropout on 16 x 76 x 76 x 255 f16: forward 83 us, 39 without dropout).
 template <int V>
 __device__ __forceinline__ void drop_apply(const DropKey& key, int q, float scale, unsigned long long e, float* f) {
     const u32x4 w = drop_words(key, e >> 3);

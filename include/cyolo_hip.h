@@ -322,7 +322,7 @@ int cy_bn_act_bwd_apply(const void* x, int ldx, const void* dy, int lddy, void* 
  *   y = res + drop(act(gamma[c] * (x - mean) * r + beta[c]))
  * The same function in training and in eval mode; stats (may be NULL: eval) receives (mean, r) as float [N][groups][2], 8-byte
  * aligned, for the backward pass.  res may be NULL.  Any C divisible by groups, any row strides >= C, any element-aligned pointer
- * (rows that all start on 16 bytes are moved 16 bytes at a time).  y may be x (every element is read before it is written by the same
+ * (rows that all start on 16 bytes are moved 16 bytes at a time).  Sums of squares are 32-bit: |x - mean| up to about 1e18.  y may be x (every element is read before it is written by the same
  * thread); no other overlap.  N = 0 or HW = 0: nothing to do.
  * Dropout (see cy_dropout): q > 0 drops with probability q / 65536, rng / id as there; element index = ((n * HW + pixel) * C + c).
  * ws: cy_gn_workspace() bytes, 8-byte aligned, ZEROED ONCE by the caller; calls of any shape may share one that is large enough for
