@@ -8,7 +8,8 @@
 // This file: the choice of kernels, the C entry points, and the general kernels -- three launches per direction: partial sums per
 // (image, pixel range, column), a fold, the element pass -- for any row stride, alignment and channel count (16 x 304 x 304 x 64 f16
 // backward 191 us in three launches, 171 in one and the parameter gradients'; 32 x 76 x 76 x 256 bf16 with a shortcut forward 68 and 64;
-// 1 x 1216 x 1216 x 32 f16, which only they take, 64 forward and 97 backward).  The one-launch kernels are in gn_resident*.  No floating-point atomics anywhere: a call's results do not depend on scheduling.
+// 1 x 1216 x 1216 x 32 f16, which only they take, 64 forward and 97 backward).  The one-launch kernels are in gn_resident*.
+// No floating-point atomics anywhere: a call's results do not depend on scheduling.
 //
 // A block works on one image n, one span of chunk columns and one range of pixels; thread = (row = t / width, chunk = t % width).
 #include "gn_math.hpp"

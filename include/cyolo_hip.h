@@ -191,7 +191,7 @@ int64_t cy_pipe_launches(void);
  * BN statistics into shared bins or the eval-mode epilogue.  CY_CONV_TILE(1) or CY_CONV_DIRECT=0 in the environment keep
  * a call on the implicit-GEMM kernels. */
 int64_t cy_direct_launches(void);
-/* Test / tool switch of the calling thread, not used on the step path.  mode 0: never use the pipelined kernel, 1: default (hints and the
+/* Test / tool switch, not used on the step path.  mode 0: never use the pipelined kernel, 1: default (hints and the
  * eval-mode epilogue select it), 2: every launch that qualifies; cap x bn (0 x 0 = policy) forces a tile capacity out of
  * {384,256,192,128} x 128 / {384,256,128} x 64 with bm_eff (0 = cap) pixels of it used; variant 0: shipped (3-stage ring,
  * LDS-transposed stores), 1: direct stores from the MFMA layout (what CY_CONV_ACCUM launches use), 2: 2-stage ring,
@@ -322,8 +322,8 @@ int cy_bn_act_bwd_apply(const void* x, int ldx, const void* dy, int lddy, void* 
  *   y = res + drop(act(gamma[c] * (x - mean) * r + beta[c]))
  * The same function in training and in eval mode; stats (may be NULL: eval) receives (mean, r) as float [N][groups][2], 8-byte
  * aligned, for the backward pass.  res may be NULL.  Any C divisible by groups, any row strides >= C, any element-aligned pointer
- * (rows that all start on 16 bytes are moved 16 bytes at a time).  Sums of squares are 32-bit: |x - mean| up to about 1e18.  y may be x (every element is read before it is written by the same
- * thread); no other overlap.  N = 0 or HW = 0: nothing to do.
+ * (rows that all start on 16 bytes are moved 16 bytes at a time).  Sums of squares are 32-bit: |x - mean| up to about 1e18.  y may
+ * be x (every element is read before it is written by the same thread); no other overlap.  N = 0 or HW = 0: nothing to do.
  * Dropout (see cy_dropout): q > 0 drops with probability q / 65536, rng / id as there; element index = ((n * HW + pixel) * C + c).
  * ws: cy_gn_workspace() bytes, 8-byte aligned, ZEROED ONCE by the caller; calls of any shape may share one that is large enough for
  * each, one after the other (calls that may run at the same time -- other streams, captured graphs among them -- need one each).
@@ -340,11 +340,11 @@ int cy_gn_act_bwd(const void* x, int ldx, const void* dy, int lddy, void* dx, in
                   void* ws, int64_t ws_bytes, cy_stream_t s);
 /* Bytes of ws for either call. */
 int64_t cy_gn_workspace(int N, int64_t HW, int C, int groups, int dtype);
-/* Test / tool switch of the calling thread, not used on the step path.  mode 0: the three-launch kernels always, 1: default (one launch where an image's
- * blocks can meet); polls: how often a block of the one-launch kernels looks for the others before it leaves its pixels to the last of
- * them (-1: default; 0: never waits); width > 0: columns of a block where the shape allows (of 16 bytes, or of one element where rows do
- * not start on 16 bytes); chunks 16 / 8: as much as a thread can hold / half of it (0: own policy).  A workspace is sized for the setting
- * it was asked under and for the default one. */
+/* Test / tool switch of the calling thread, not used on the step path.  mode 0: the three-launch kernels always, 1: default (one
+ * launch where an image's blocks can meet); polls: how often a block of the one-launch kernels looks for the others before it leaves
+ * its pixels to the last of them (-1: default; 0: never waits); width > 0: columns of a block where the shape allows (of 16 bytes, or of
+ * one element where rows do not start on 16 bytes); chunks 16 / 8: as much as a thread can hold / half of it (0: own policy).  A
+ * workspace is sized for the setting it was asked under and for the default one. */
 int cy_gn_config(int mode, int polls, int width, int chunks);
 /* Test / tool query: what a call of this shape would run under the thread's setting, rows16: every row of every operand starts on 16
  * bytes.  plan[6] = launches (1 or 3; the parameter gradients' not counted), columns of a block, chunks a thread holds (0: three
